@@ -6,6 +6,7 @@ message on failure.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import functools
 import threading
@@ -54,6 +55,21 @@ class ExpertBank(C.Structure):
         "int8_w2_scales", "int4_w13", "int4_w13_scales", "int4_w2", "int4_w2_scales")]
 
 
+class RouteProblem(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("n_tokens", "n_experts", "top_k", "n_groups",
+                                         "topk_group")] + \
+               [(n, C.c_int) for n in ("logits_dtype", "bias_dtype", "ids_dtype",
+                                       "weights_dtype", "scoring", "group_score",
+                                       "renormalize")] + [("scale", C.c_float)]
+
+
+class LinearProblem(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("n_tokens", "in_features", "out_features", "x_stride",
+                                         "weight_stride", "residual_stride", "out_stride")] + \
+               [(n, C.c_int) for n in ("act_dtype", "bias_dtype", "residual_dtype", "out_dtype",
+                                       "activation", "gated")]
+
+
 _P, _I64, _INT, _SZ = C.c_void_p, C.c_int64, C.c_int, C.c_size_t
 
 _SIGNATURES = {
@@ -62,6 +78,8 @@ _SIGNATURES = {
     "exq_status_name": ([_INT], C.c_char_p),
     "exq_moe_align_block_size": ([_P, _INT, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _INT, _P], _INT),
     "exq_topk_softmax": ([_P, _INT, _I64, _I64, _I64, _INT, _P, _INT, _P, _INT, _P], _INT),
+    "exq_grouped_topk": ([C.POINTER(RouteProblem), _P, _P, _P, _P, _P, _P], _INT),
+    "exq_linear": ([C.POINTER(LinearProblem), _P, _P, _P, _P, _P, _P], _INT),
     "exq_build_ends_from_slots": ([_P, _I64, _P, _I64, _I64, _P, _P, _P], _INT),
     "exq_dispatch": ([_P, _INT, _I64, _I64, _P, _P, _P, _P], _INT),
     "exq_gather_hidden": ([_P, _INT, _I64, _I64, _P, _I64, _I64, _P, _P], _INT),
@@ -137,6 +155,17 @@ def stream_handle(device: torch.device) -> int:
     # (1.5 us of a call that takes 12 on the GPU)
     i = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if i is None else i)
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` the current one for a launch, where it is not."""
+    i = device.index
+    if i is None or i == torch._C._cuda_getDevice():
+        return _NO_SWITCH
+    return torch.cuda.device(device)
 
 
 def require_gpu(*tensors: torch.Tensor) -> torch.device:

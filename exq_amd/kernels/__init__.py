@@ -10,7 +10,8 @@ from .moe_grouped_gemm import moe_grouped_gemm, sort_tokens_by_expert, unsort_ou
 from .moe_int4_kernel import (moe_int4_forward, moe_int4_full_forward, pack_experts_int4,
                               pack_int4_weights)
 from . import exq_dispatch
-from .exq_dispatch import fused_topk
+from .exq_dispatch import fused_topk, grouped_topk
+from .linear import fused_gated_linear, fused_linear
 from .quant_shim import quantize_tensor_int4, quantize_tensor_int8
 
 __all__ = [
@@ -29,6 +30,9 @@ __all__ = [
     "quantize_int8_rows",
     "exq_dispatch",
     "fused_topk",
+    "grouped_topk",
+    "fused_linear",
+    "fused_gated_linear",
     "quantize_tensor_int4",
     "quantize_tensor_int8",
 ]

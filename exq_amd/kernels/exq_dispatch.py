@@ -171,3 +171,82 @@ def fused_topk(gating_output: torch.Tensor, topk: int, renormalize: bool,
                                   _lib.dtype_code(wts.dtype), _lib.stream_handle(dev)),
                "fused_topk")
     return wts, ids
+
+
+_SCORING = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORE = {"max": 0, "top2": 1}
+_FLOAT_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def grouped_topk(gating_output: torch.Tensor, topk: int, renormalize: bool,
+                 num_expert_group: int = 1, topk_group: int = 1, *,
+                 scoring_func: str = "softmax", correction_bias: torch.Tensor | None = None,
+                 group_score: str | None = None, routed_scaling_factor: float = 1.0,
+                 num_token_non_padded: torch.Tensor | None = None,
+                 ids_dtype: torch.dtype = torch.int32,
+                 weights_dtype: torch.dtype = torch.float32):
+    """Router with groups of experts, one kernel: softmax or sigmoid scores of
+    ``gating_output`` [T, E], ranked by score + ``correction_bias`` [E] (a balancing
+    bias; it ranks and never weighs), the ``topk_group`` best of ``num_expert_group``
+    groups of consecutive experts, and the ``topk`` best experts in those.
+
+    Returns ``(topk_weights [T, k], topk_ids [T, k])`` like ``fused_topk``: the
+    scores of the chosen, divided by their sum when ``renormalize``, times
+    ``routed_scaling_factor``; ids in descending order of the ranking, equal values
+    to the lower id (equal groups to the lower group).  The ranking is that of the
+    scores in 64 bits, whatever the logits' type.  ``group_score``: a group is worth
+    its best expert ("max", the default without a bias) or the sum of its two best
+    ("top2", the default with one).
+
+    Logits or biases of -inf or NaN mask an expert: it has no part in the softmax,
+    the group's value or the choice; a logit of +inf counts as the largest finite
+    float32.  Slots that no expert is left for get id -1, which the expert layers
+    drop, and weight 0; so do all slots of the rows from ``num_token_non_padded``
+    (int32, one element on the device) on, the padding of a captured batch.
+    Stream-ordered, graph-capturable, no workspace, no backward.
+    """
+    if gating_output.dim() != 2:
+        raise ValueError("gating_output must be [T, E]")
+    if gating_output.dtype not in _FLOAT_DTYPES:
+        raise ValueError("gating_output must be float32, float16 or bfloat16")
+    T, E = gating_output.shape
+    if not 1 <= E <= 1024:
+        raise ValueError(f"E={E} experts is not in [1, 1024]")
+    if not 1 <= num_expert_group <= 64 or E % num_expert_group:
+        raise ValueError(f"num_expert_group={num_expert_group} must divide E={E} and be at most 64")
+    if not 1 <= topk_group <= num_expert_group:
+        raise ValueError(f"topk_group={topk_group} must be in [1, num_expert_group]")
+    if not 1 <= topk <= min(64, E // num_expert_group * topk_group):
+        raise ValueError(f"topk={topk} must be in [1, 64] and fit the experts of topk_group groups")
+    if scoring_func not in _SCORING:
+        raise ValueError(f"unsupported scoring_func {scoring_func!r}")
+    if group_score is None:
+        group_score = "max" if correction_bias is None else "top2"
+    if group_score not in _GROUP_SCORE:
+        raise ValueError(f"unsupported group_score {group_score!r}")
+    if ids_dtype not in (torch.int32, torch.int64) or weights_dtype not in _FLOAT_DTYPES:
+        raise ValueError("ids must be int32 or int64, weights float32, float16 or bfloat16")
+    if correction_bias is not None and (correction_bias.dtype not in _FLOAT_DTYPES
+                                        or tuple(correction_bias.shape) != (E,)):
+        raise ValueError(f"correction_bias must be [{E}], float32, float16 or bfloat16")
+    if num_token_non_padded is not None and (num_token_non_padded.dtype != torch.int32
+                                             or num_token_non_padded.numel() != 1):
+        raise ValueError("num_token_non_padded must be one int32 element on the device")
+    if torch.is_grad_enabled() and (gating_output.requires_grad or (
+            correction_bias is not None and correction_bias.requires_grad)):
+        raise ValueError("grouped_topk has no backward: call it under torch.no_grad()")
+    g = gating_output if gating_output.is_contiguous() else gating_output.contiguous()
+    dev = _lib.require_gpu(g, correction_bias, num_token_non_padded)
+    ids = torch.empty(T, topk, dtype=ids_dtype, device=dev)
+    wts = torch.empty(T, topk, dtype=weights_dtype, device=dev)
+    code = _lib._TORCH_TO_CODE
+    p = _lib.RouteProblem(T, E, topk, num_expert_group, topk_group, code[g.dtype],
+                          0 if correction_bias is None else code[correction_bias.dtype],
+                          code[ids_dtype], code[weights_dtype], _SCORING[scoring_func],
+                          _GROUP_SCORE[group_score], 1 if renormalize else 0,
+                          routed_scaling_factor)
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().exq_grouped_topk(
+            p, g.data_ptr(), _lib.ptr(correction_bias), _lib.ptr(num_token_non_padded),
+            ids.data_ptr(), wts.data_ptr(), _lib.stream_handle(dev)), "grouped_topk")
+    return wts, ids

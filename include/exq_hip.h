@@ -83,6 +83,47 @@ int exq_topk_softmax(const void* logits, int logits_dtype, int64_t n_tokens,
                      int ids_dtype, void* topk_weights, int weights_dtype, exq_stream stream);
 
 /*
+ * Router with groups of experts: scores of logits [T, E] by softmax over the
+ * experts or by sigmoid, ranked by score + bias[e] (bias nullable), restricted to
+ * the topk_group best of n_groups groups of E / n_groups consecutive experts (a
+ * group is worth its best expert, or the sum of its two best), the k best experts
+ * of those -> topk_ids, topk_weights [T, k].  Weights are the scores without the
+ * bias, divided by their sum when renormalize != 0, times scale.  Ids are in
+ * descending order of the ranking, equal values to the lower id, and equal groups
+ * to the lower group; the ranking is that of the scores in 64 bits.  No counterpart
+ * in the reference, whose router is exq_topk_softmax's
+ * (exq/codegen/triton_emitter.py:273-277).
+ * An expert whose logit or bias is -inf or NaN is masked: it has no part in the
+ * softmax, in its group's value and in the choice; a logit of +inf counts as the
+ * largest finite float.  Slots for which no expert is left get id -1 (dropped by
+ * the layers) and weight 0, and so do all slots of the rows from *n_valid on
+ * (nullable, a device value: the padding of a captured batch).
+ * n_experts <= 1024, n_groups <= 64, top_k <= 64.  No workspace.
+ */
+typedef enum exq_scoring { EXQ_SCORE_SOFTMAX = 0, EXQ_SCORE_SIGMOID = 1 } exq_scoring;
+typedef enum exq_group_score { EXQ_GROUP_MAX = 0, EXQ_GROUP_TOP2 = 1 } exq_group_score;
+
+typedef struct exq_route_problem {
+  int64_t n_tokens;
+  int64_t n_experts;
+  int64_t top_k;
+  int64_t n_groups;      /* divides n_experts */
+  int64_t topk_group;    /* groups that stay */
+  int logits_dtype;      /* f32 | f16 | bf16 */
+  int bias_dtype;        /* f32 | f16 | bf16 */
+  int ids_dtype;         /* i32 | i64 */
+  int weights_dtype;     /* f32 | f16 | bf16 */
+  int scoring;           /* exq_scoring */
+  int group_score;       /* exq_group_score */
+  int renormalize;
+  float scale;
+} exq_route_problem;
+
+int exq_grouped_topk(const exq_route_problem* problem, const void* logits, const void* bias,
+                     const int32_t* n_valid, void* topk_ids, void* topk_weights,
+                     exq_stream stream);
+
+/*
  * Block-padded expert layout.  Replaces sgl_kernel.moe_align_block_size as
  * called at exq/runtime/sglang_backend.py:102-109 (num_experts = E + 1,
  * block_size = 16).  Bucket b = id + 1 (bucket 0 collects id == -1);
@@ -231,6 +272,49 @@ int exq_moe_routed_gemm(const void* hidden, int act_dtype, int64_t n_tokens, int
                         int64_t n_experts, int64_t N, int64_t group_size,
                         const int32_t* expert_mask, void* c, void* workspace,
                         size_t workspace_bytes, exq_stream stream);
+
+/* ---- products with an epilogue -------------------------------------------- */
+
+typedef enum exq_activation {
+  EXQ_ACT_NONE = 0,
+  EXQ_ACT_RELU = 1,
+  EXQ_ACT_SILU = 2,
+  EXQ_ACT_GELU = 3,       /* x / 2 * (1 + erf(x / sqrt 2)) */
+  EXQ_ACT_GELU_TANH = 4,  /* x / 2 * (1 + tanh(sqrt(2 / pi) * (x + 0.044715 x^3))) */
+  EXQ_ACT_SIGMOID = 5
+} exq_activation;
+
+typedef struct exq_linear_problem {
+  int64_t n_tokens;        /* T */
+  int64_t in_features;     /* K */
+  int64_t out_features;    /* N: columns of out */
+  int64_t x_stride;        /* elements from row to row of x, W, residual and out */
+  int64_t weight_stride;
+  int64_t residual_stride;
+  int64_t out_stride;      /* at least N when T > 1 */
+  int act_dtype;           /* x and W: f16 | bf16 */
+  int bias_dtype;          /* f32 | f16 | bf16 */
+  int residual_dtype;      /* f32 | f16 | bf16 */
+  int out_dtype;           /* f32 | f16 | bf16 */
+  int activation;          /* exq_activation */
+  int gated;               /* 0 | 1 */
+} exq_linear_problem;
+
+/*
+ * Dense product with its epilogue, for what stands beside the routed experts: the
+ * router's projection, shared experts, dense layers.
+ *   gated = 0: out = act(x @ W^T + bias) + residual, W [N, K], bias [N]
+ *   gated = 1: out = act(x @ Wg^T + bg) * (x @ Wu^T + bu), W [2N, K] and bias [2N]
+ *              with the N gate rows first (as w13), no residual
+ * x [T, K], residual and out [T, N]; bias and residual may be null.  Products are
+ * summed in fp32 and the result is rounded once, to out_dtype.  Rows are
+ * contiguous, their strides free (0 repeats a row of an input).  out may be
+ * residual itself (same pointer, dtype and stride) and must not overlap any other
+ * input.  Any sizes: K and N need no alignment (16-byte aligned rows run on the
+ * faster kernels).  No workspace, no counterpart in the reference.
+ */
+int exq_linear(const exq_linear_problem* problem, const void* x, const void* weight,
+               const void* bias, const void* residual, void* out, exq_stream stream);
 
 /* ---- weight quantisation -------------------------------------------------- */
 

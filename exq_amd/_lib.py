@@ -6,7 +6,6 @@ message on failure.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import functools
 import threading
@@ -157,15 +156,27 @@ def stream_handle(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if i is None else i)
 
 
-_NO_SWITCH = contextlib.nullcontext()
+@functools.lru_cache(maxsize=4096)
+def route_problem(*fields) -> RouteProblem:
+    """The problem of a grouped_topk call, which the library only reads."""
+    return RouteProblem(*fields)
 
 
-def on_device(device: torch.device):
-    """Makes ``device`` the current one for a launch, where it is not."""
-    i = device.index
-    if i is None or i == torch._C._cuda_getDevice():
-        return _NO_SWITCH
-    return torch.cuda.device(device)
+@functools.lru_cache(maxsize=4096)
+def linear_problem(*fields) -> LinearProblem:
+    """The problem of a fused_linear call, which the library only reads."""
+    return LinearProblem(*fields)
+
+
+def launch(entry, args: tuple, index: int, what: str) -> None:
+    """``entry(*args, stream)`` on the current stream of device ``index``, which is made
+    the current device for the call where it is not."""
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return launch(entry, args, index, what)
+    status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status, what)
 
 
 def require_gpu(*tensors: torch.Tensor) -> torch.device:

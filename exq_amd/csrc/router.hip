@@ -26,6 +26,8 @@ struct RouteArgs {
   int ldt, bdt, idt, wdt;
   int T, E, k, G, gs, top_groups;
   int sigmoid, top2, renorm;
+  int chunk, vec;            // experts of a lane; runs of four may be loaded at once
+  int lanes2, chunk2;        // lanes of a kept group, and experts of a lane then
   float scale;
 };
 
@@ -45,52 +47,32 @@ __device__ __forceinline__ uint32_t wave_reduce(uint32_t v, Op op) {
   v = op(v, dpp<0x143, 0xc, ID>(v));  // row_bcast 31 -> rows 2, 3
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-  return wave_reduce<0u>(v, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
-}
 __device__ __forceinline__ uint32_t wave_min(uint32_t v) {
   return wave_reduce<0xffffffffu>(v, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
 }
-__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
-  const uint32_t hi = wave_max((uint32_t)(v >> 32));
-  const uint32_t lo = wave_max((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
-  return (uint64_t)hi << 32 | lo;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dppd(double v) {  // (-inf in lanes that the step leaves out)
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = dpp<CTRL, ROWS, 0u>((uint32_t)u);
+  const uint32_t hi = dpp<CTRL, ROWS, 0xfff00000u>((uint32_t)(u >> 32));
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ double wave_max64(double v) {
+  v = fmax(v, dppd<0xB1, 0xf>(v));
+  v = fmax(v, dppd<0x4E, 0xf>(v));
+  v = fmax(v, dppd<0x124, 0xf>(v));
+  v = fmax(v, dppd<0x128, 0xf>(v));
+  v = fmax(v, dppd<0x142, 0xa>(v));
+  v = fmax(v, dppd<0x143, 0xc>(v));
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
   return v;
-}
-
-// Order-preserving key of a rank value (-0 and +0 share one); 0 lies below every
-// key and marks an expert that is not there, or taken.
-__device__ __forceinline__ uint64_t rank_key(double r) {
-  uint64_t b = (uint64_t)__double_as_longlong(r);
-  if ((b << 1) == 0u) b = 0u;
-  return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
-}
-__device__ __forceinline__ double key_rank(uint64_t k) {
-  return __longlong_as_double((long long)((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k));
-}
-
-// The best remaining key of the wave and its expert (lane l holds experts l + 64 c):
-// the lowest id among equal keys.  Key 0: none is left.
-template <int MAXC>
-__device__ __forceinline__ uint64_t wave_best(const uint64_t (&key)[MAXC], int lane, int lo,
-                                              int hi, int& expert) {
-  uint64_t bk = 0u;
-  int be = 0;
-#pragma unroll
-  for (int c = 0; c < MAXC; ++c) {
-    const int e = lane + 64 * c;
-    if (e >= lo && e < hi && key[c] > bk) {  // strict: the lower id keeps a tie
-      bk = key[c];
-      be = e;
-    }
-  }
-  const uint64_t K = wave_max64(bk);
-  expert = (int)wave_min(bk == K && K ? (uint32_t)be : 0xffffffffu);
-  return K;
 }
 
 __device__ __forceinline__ void store_choice(const RouteArgs& a, int64_t row, int j, int id,
@@ -104,13 +86,14 @@ __device__ __forceinline__ void store_choice(const RouteArgs& a, int64_t row, in
 }
 
 // One token, by one wave, ranked in 64 bits: neither an expert nor a group is
-// decided by the rounding of a score.  The weights are the chosen scores:
-// exp(u - U) / sum with u = l (softmax) or log(sigmoid(l)) = min(l, 0) -
+// decided by the rounding of a score.  Lane l holds experts l + 64 c; `mem` is E doubles
+// of the wave's own LDS, used where groups are chosen.  The weights are the chosen
+// scores: exp(u - U) / sum with u = l (softmax) or log(sigmoid(l)) = min(l, 0) -
 // log1p(exp(-|l|)), and U the largest chosen u where they are renormalised, so
 // that scores which all underflow still have their ratio.
 template <int MAXC>
-__device__ void route_row(const RouteArgs& a, int64_t row, int lane) {
-  uint64_t key[MAXC];
+__device__ void route_row(const RouteArgs& a, int64_t row, int lane, double* mem) {
+  double r[MAXC];  // rank values, -inf where an expert is masked or taken
   float lg[MAXC];
   float m = -FLT_MAX;
 #pragma unroll
@@ -126,75 +109,87 @@ __device__ void route_row(const RouteArgs& a, int64_t row, int lane) {
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+  const bool by_sum = a.top_groups < a.G && a.top2;
   double S = 0.0;
   if (!a.sigmoid) {
 #pragma unroll
-    for (int c = 0; c < MAXC; ++c)
-      if (lg[c] > -INFINITY) S += exp((double)lg[c] - (double)m);
+    for (int c = 0; c < MAXC; ++c) {
+      r[c] = lg[c] > -INFINITY ? exp((double)lg[c] - (double)m) : 0.0;
+      S += r[c];
+    }
     S = wave_sum64(S);
+  } else if (a.bias || by_sum) {
+#pragma unroll
+    for (int c = 0; c < MAXC; ++c) r[c] = 1.0 / (1.0 + exp(-(double)lg[c]));
   }
 #pragma unroll
   for (int c = 0; c < MAXC; ++c) {
-    key[c] = 0u;
-    if (lg[c] > -INFINITY) {
-      double r = lg[c];
-      if (a.bias) {
-        const double s = a.sigmoid ? 1.0 / (1.0 + exp(-(double)lg[c]))
-                                   : exp((double)lg[c] - (double)m) / S;
-        r = s + (double)load_as_f32(a.bias, a.bdt, lane + 64 * c);
-      }
-      key[c] = rank_key(r);
-    }
+    const int e = lane + 64 * c;
+    const bool there = lg[c] > -INFINITY;
+    const double s = a.sigmoid ? r[c] : r[c] / S;
+    if (by_sum && !a.bias && e < a.E) mem[e] = there ? s : -INFINITY;
+    r[c] = !there ? -INFINITY : a.bias ? s + (double)load_as_f32(a.bias, a.bdt, e) : (double)lg[c];
+    if (a.top_groups < a.G && !(by_sum && !a.bias) && e < a.E) mem[e] = r[c];
   }
 
   if (a.top_groups < a.G) {
-    // lane g: the value of group g
-    uint64_t gkey = 0u;
-    for (int g = 0; g < a.G; ++g) {
-      int e1, e2;
-      const int lo = g * a.gs, hi = lo + a.gs;
-      uint64_t v = wave_best<MAXC>(key, lane, lo, hi, e1);
-      if (a.top2 && v) {
-        // the two best scores, not the logits that rank them where there is no bias
-        uint64_t rest[MAXC];
+    // lane g: the value of group g, and how many groups come before it
+    __builtin_amdgcn_wave_barrier();
+    double v1 = -INFINITY, v2 = -INFINITY;
+    if (lane < a.G) {
+      auto take = [&](double x) {
+        v2 = fmax(v2, fmin(v1, x));
+        v1 = fmax(v1, x);
+      };
+      const double* at = mem + lane * a.gs;
+      int i = 0;
+      for (; i + 8 <= a.gs; i += 8) {  // (eight reads in flight)
+        double x[8];
 #pragma unroll
-        for (int c = 0; c < MAXC; ++c) rest[c] = lane + 64 * c == e1 ? 0u : key[c];
-        const uint64_t v2 = wave_best<MAXC>(rest, lane, lo, hi, e2);
-        double r1 = key_rank(v), r2 = v2 ? key_rank(v2) : 0.0;
-        if (!a.bias) {
-          r1 = a.sigmoid ? 1.0 / (1.0 + exp(-r1)) : exp(r1 - (double)m) / S;
-          if (v2) r2 = a.sigmoid ? 1.0 / (1.0 + exp(-r2)) : exp(r2 - (double)m) / S;
-        }
-        v = rank_key(r1 + r2);
+        for (int q = 0; q < 8; ++q) x[q] = at[i + q];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) take(x[q]);
       }
-      if (lane == g) gkey = v;
+      for (; i < a.gs; ++i) take(at[i]);
     }
-    uint64_t keep = 0u;
-    for (int j = 0; j < a.top_groups; ++j) {
-      const uint64_t K = wave_max64(gkey);
-      if (K == 0u) break;
-      const int g = (int)wave_min(gkey == K ? (uint32_t)lane : 0xffffffffu);
-      keep |= 1ull << g;
-      if (lane == g) gkey = 0u;
+    if (a.top2 && v2 > -INFINITY) v1 = v1 + v2;
+    int before = 0;
+#pragma unroll 4
+    for (int g = 0; g < a.G; ++g) {
+      const double o = __shfl(v1, g, 64);
+      before += o > v1 || (o == v1 && g < lane) ? 1 : 0;
     }
+    const uint64_t keep = __ballot(lane < a.G && before < a.top_groups);
 #pragma unroll
     for (int c = 0; c < MAXC; ++c) {
       const int e = lane + 64 * c;
-      if (e < a.E && !(keep >> (e / a.gs) & 1u)) key[c] = 0u;
+      if (e < a.E && !(keep >> (e / a.gs) & 1u)) r[c] = -INFINITY;
     }
   }
 
   int my_id = -1;
   float my_l = -INFINITY;
   for (int j = 0; j < a.k; ++j) {
-    int e;
-    const uint64_t K = wave_best<MAXC>(key, lane, 0, a.E, e);
-    if (K == 0u) break;
+    double bv = -INFINITY;
+    int be = 0;
+#pragma unroll
+    for (int c = 0; c < MAXC; ++c)
+      if (r[c] > bv) {  // strict: the lower id keeps a tie
+        bv = r[c];
+        be = lane + 64 * c;
+      }
+    const double M = wave_max64(bv);
+    if (M == -INFINITY) break;
+    const uint64_t at = __ballot(bv == M);
+    const int e = __popcll(at) == 1
+                      ? __builtin_amdgcn_readlane(
+                            be, __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)at) - 1))
+                      : (int)wave_min(bv == M ? (uint32_t)be : 0xffffffffu);
     float l = 0.f;
 #pragma unroll
     for (int c = 0; c < MAXC; ++c)
       if (lane + 64 * c == e) {
-        key[c] = 0u;
+        r[c] = -INFINITY;
         l = lg[c];
       }
     l = __shfl(l, e & 63, 64);
@@ -209,9 +204,7 @@ __device__ void route_row(const RouteArgs& a, int64_t row, int lane) {
     if (a.sigmoid) w = fmin(w, 0.0) - log1p(exp(-fabs(w)));
   }
   if (a.renorm) {
-    double U = my_id >= 0 ? w : -INFINITY;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) U = fmax(U, __shfl_xor(U, d, 64));
+    const double U = wave_max64(my_id >= 0 ? w : -INFINITY);
     w = my_id >= 0 ? exp(w - U) : 0.0;
     const double sum = wave_sum64(w);
     w = my_id >= 0 ? w / sum : 0.0;
@@ -223,14 +216,386 @@ __device__ void route_row(const RouteArgs& a, int64_t row, int lane) {
 
 template <int MAXC>
 __global__ void __launch_bounds__(256) route_rows_kernel(RouteArgs a) {
+  __shared__ double s_mem[4][64 * MAXC];
   const int lane = threadIdx.x & 63;
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.T) return;  // (wave-uniform)
+  if (row >= a.T) return;  // (wave-uniform; the waves never meet)
   if (a.n_valid && row >= *a.n_valid) {
     if (lane < a.k) store_choice(a, row, lane, -1, 0.f);
     return;
   }
-  route_row<MAXC>(a, row, lane);
+  route_row<MAXC>(a, row, lane, s_mem[threadIdx.x >> 6]);
+}
+
+// ---- four tokens a wave ------------------------------------------------------------
+// A token is a 16-lane row of the wave.  Scores in fp32; what their roundings could
+// decide, the wave ranks again in 64 bits (route_row).  In order:
+//   the groups, 16 / G lanes each: their values by butterflies over their lanes, each
+//     one's rank by counting, row rotations against all others; the keys of the kept
+//     groups are dealt out again over all lanes, through LDS;
+//   a threshold: the k + 1-th best of the lanes' two best keys, which at least k + 1
+//     experts reach, and rarely many more;
+//   the experts that reach it, packed into 16 KC slots of LDS, and their ranks by
+//     counting again: no round per choice, and no lane is searched twice.
+template <int CTRL>
+__device__ __forceinline__ float rowf(float v) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ int rowi(int v) {
+  return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true);
+}
+// Every lane of an aligned run of N lanes gets the run's reduction: pairs, quads, then
+// mirrored halves of lanes that agree within them.
+template <int N, typename Op>
+__device__ __forceinline__ float row_reduce(float v, Op op) {
+  if constexpr (N >= 2) v = op(v, rowf<0xB1>(v));
+  if constexpr (N >= 4) v = op(v, rowf<0x4E>(v));
+  if constexpr (N >= 8) v = op(v, rowf<0x141>(v));
+  if constexpr (N >= 16) v = op(v, rowf<0x140>(v));
+  return v;
+}
+__device__ __forceinline__ float max_op(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float min_op(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ float sum_op(float a, float b) { return a + b; }
+// f(constant I), ... f(constant N - 1)
+template <int I, int N, typename F>
+__device__ __forceinline__ void unrolled(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    unrolled<I + 1, N>(f);
+  }
+}
+
+struct Candidate {
+  float key;
+  int id;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Four consecutive values of a float-typed array, aligned to their size.
+__device__ __forceinline__ float4 load4(const void* p, int dt, int64_t i) {
+  if (dt == EXQ_DTYPE_F32)
+    return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+  const uint2 u = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + i);
+  if (dt == EXQ_DTYPE_BF16)
+    return float4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
+                  __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u)};
+  return float4{f16_bits_to_f32(u.x & 0xffffu), f16_bits_to_f32(u.x >> 16),
+                f16_bits_to_f32(u.y & 0xffffu), f16_bits_to_f32(u.y >> 16)};
+}
+
+// The k best of a row's keys, lane l holding those of experts e0 .. e0 + CH - 1 (-inf:
+// none): candidates c[i] with their ranks, slot i * 16 + l of `total`.
+template <int CH, int KC>
+__device__ __forceinline__ void rank_experts(const float (&key)[CH], int e0, int k, int lane,
+                                             Candidate* cand, Candidate (&c)[KC], int (&rank)[KC],
+                                             int& total) {
+  const int l16 = lane & 15;
+  // V: the largest of the lanes' two best that k + 1 of them reach
+  float m1 = -INFINITY, m2 = -INFINITY;
+#pragma unroll
+  for (int p = 0; p < CH; ++p) {
+    m2 = fmaxf(m2, fminf(m1, key[p]));
+    m1 = fmaxf(m1, key[p]);
+  }
+  int c1 = m2 >= m1 ? 2 : 1, c2 = 2;
+  unrolled<1, 16>([&](auto j) {
+    constexpr int CTRL = 0x120 + decltype(j)::value;  // rotate the row
+    const float o1 = rowf<CTRL>(m1), o2 = rowf<CTRL>(m2);
+    c1 += (o1 >= m1 ? 1 : 0) + (o2 >= m1 ? 1 : 0);
+    c2 += (o1 >= m2 ? 1 : 0) + (o2 >= m2 ? 1 : 0);
+  });
+  float V = row_reduce<16>(c1 > k ? m1 : c2 > k ? m2 : -INFINITY, max_op);
+  V = fmaxf(V, -FLT_MAX);  // (an expert that is there has a key above -inf)
+  int cnt = 0;
+#pragma unroll
+  for (int p = 0; p < CH; ++p) cnt += key[p] >= V ? 1 : 0;
+  int upto = cnt;  // inclusive prefix over the row (row_shr, zeros shifted in)
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xf, 0xf, false);
+  total = __shfl(upto, lane | 15, 64);
+  int at = upto - cnt;
+#pragma unroll
+  for (int p = 0; p < CH; ++p)
+    if (key[p] >= V) {
+      if (at < 16 * KC) cand[at] = Candidate{key[p], e0 + p};
+      ++at;
+    }
+  __builtin_amdgcn_wave_barrier();  // (the wave's own LDS, in order)
+#pragma unroll
+  for (int i = 0; i < KC; ++i) {
+    const int slot = i * 16 + l16;
+    c[i] = slot < total ? cand[slot] : Candidate{-INFINITY, 4096 + slot};
+    rank[i] = 0;
+  }
+  auto first_of = [](float ok, int oid, const Candidate& x) {
+    return ok > x.key || (ok == x.key && oid < x.id) ? 1 : 0;
+  };
+#pragma unroll
+  for (int i = 0; i < KC; ++i)
+#pragma unroll
+    for (int j = 0; j < KC; ++j)
+      if (i != j) rank[i] += first_of(c[j].key, c[j].id, c[i]);
+  unrolled<1, 16>([&](auto r) {
+    constexpr int CTRL = 0x120 + decltype(r)::value;
+#pragma unroll
+    for (int j = 0; j < KC; ++j) {
+      const float ok = rowf<CTRL>(c[j].key);
+      const int oid = rowi<CTRL>(c[j].id);
+#pragma unroll
+      for (int i = 0; i < KC; ++i) rank[i] += first_of(ok, oid, c[i]);
+    }
+  });
+}
+
+// Roundings.  In units of 2^-24: e^x as exp2(x log2 e) is off by 2.5 |x| + 2 of itself,
+// and |x| e^-|x| <= 0.37, x s (1 - s) <= 0.23, so a sigmoid s is off by at most 4 and e / S
+// by 3 / S + 58 s (S: a weighted mean of |x| is at most ln 512, 36 additions); adding the
+// bias rounds once.  A ranking between two values no further apart than both bounds
+// together is left to route_row (`tol`: 9 and 128 / S for the scores, a little over 2 |r|
+// for the rounded sums); a sum of two scores has twice that.  With logits as they come
+// and a small bias that is about one row in 3,000.
+template <int CH, int G, int KC, int MAXC>
+__global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
+  constexpr int LG = 16 / G;       // lanes of a group
+  constexpr int KEYS = 16 * CH + 4;  // floats of a token's keys in LDS
+  __shared__ Candidate s_cand[16][16 * KC + 1];
+  __shared__ float s_sorted[16][16 * KC + 1];
+  __shared__ __align__(16) float s_key[G > 1 ? 16 : 1][G > 1 ? KEYS : 4];
+  const int lane = threadIdx.x & 63, l16 = lane & 15;
+  const int tok = threadIdx.x >> 4;   // token of the work-group
+  const int row0 = blockIdx.x * 16 + (threadIdx.x >> 6) * 4;  // first row of the wave
+  if (row0 >= a.T) return;            // (wave-uniform; the waves never meet)
+  const int row = blockIdx.x * 16 + tok;
+  const int64_t rr = row < a.T ? row : a.T - 1;
+  const int g = l16 / LG, sub = l16 % LG;
+  const int chunk = a.chunk, first = sub * chunk;
+  const int n = first >= a.gs ? 0 : a.gs - first < chunk ? a.gs - first : chunk;
+  int e0 = g * a.gs + first;
+
+  float l[CH], key[CH], b[CH];
+#pragma unroll
+  for (int p = 0; p < CH; ++p) {
+    l[p] = -INFINITY;
+    b[p] = 0.f;
+  }
+  if (a.vec) {  // runs of four start at multiples of four, and n is one
+#pragma unroll
+    for (int p = 0; p < CH; p += 4)
+      if (p < n) {
+        const float4 v = load4(a.logits, a.ldt, rr * a.E + e0 + p);
+        l[p] = v.x; l[p + 1] = v.y; l[p + 2] = v.z; l[p + 3] = v.w;
+        if (a.bias) {
+          const float4 u = load4(a.bias, a.bdt, e0 + p);
+          b[p] = u.x; b[p + 1] = u.y; b[p + 2] = u.z; b[p + 3] = u.w;
+        }
+      }
+  } else {
+#pragma unroll
+    for (int p = 0; p < CH; ++p)
+      if (p < n) {
+        l[p] = load_as_f32(a.logits, a.ldt, rr * a.E + e0 + p);
+        if (a.bias) b[p] = load_as_f32(a.bias, a.bdt, e0 + p);
+      }
+  }
+#pragma unroll
+  for (int p = 0; p < CH; ++p) {
+    const bool there = l[p] > -INFINITY && b[p] > -INFINITY;  // (false for NaN)
+    l[p] = p < n && there ? fminf(l[p], FLT_MAX) : -INFINITY;
+  }
+
+  // softmax: largest logit and sum, where a score of it is needed
+  float m = 0.f, S = 1.f;
+  if (!a.sigmoid && (a.bias || !a.renorm || (G > 1 && a.top2))) {
+    m = -FLT_MAX;
+#pragma unroll
+    for (int p = 0; p < CH; ++p) m = fmaxf(m, l[p]);
+    m = row_reduce<16>(m, max_op);
+    S = 0.f;
+#pragma unroll
+    for (int p = 0; p < CH; ++p) {
+      key[p] = __builtin_amdgcn_exp2f((l[p] - m) * kLog2e);  // (0 where masked)
+      S += key[p];
+    }
+    S = row_reduce<16>(S, sum_op);
+  }
+  const float rS = __builtin_amdgcn_rcpf(S);
+  auto score = [&](float x) {  // (0 for -inf)
+    return a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-x * kLog2e))
+                     : __builtin_amdgcn_exp2f((x - m) * kLog2e) * rS;
+  };
+  const float tol0 = a.sigmoid ? 0x1.2p-21f : 0x1p-17f * rS;
+  if (a.bias) {
+    if (a.sigmoid) {
+#pragma unroll
+      for (int p = 0; p < CH; ++p) key[p] = score(l[p]);
+    } else {
+#pragma unroll
+      for (int p = 0; p < CH; ++p) key[p] *= rS;
+    }
+#pragma unroll
+    for (int p = 0; p < CH; ++p) key[p] = l[p] > -INFINITY ? key[p] + b[p] : -INFINITY;
+  } else {
+#pragma unroll
+    for (int p = 0; p < CH; ++p) key[p] = l[p];
+  }
+  bool unsure = false;
+  Candidate c[KC];
+  int rank[KC], total;
+
+  if constexpr (G > 1) {
+    float v1 = -INFINITY, v2 = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < CH; ++p) {
+      v2 = fmaxf(v2, fminf(v1, key[p]));
+      v1 = fmaxf(v1, key[p]);
+    }
+    float v;
+    if (a.top2) {
+      auto merge = [&](float o1, float o2) {
+        v2 = fmaxf(fminf(v1, o1), fmaxf(v2, o2));
+        v1 = fmaxf(v1, o1);
+      };
+      if constexpr (LG >= 2) merge(rowf<0xB1>(v1), rowf<0xB1>(v2));
+      if constexpr (LG >= 4) merge(rowf<0x4E>(v1), rowf<0x4E>(v2));
+      if constexpr (LG >= 8) merge(rowf<0x141>(v1), rowf<0x141>(v2));
+      const float s1 = a.bias ? v1 : score(v1), s2 = a.bias ? v2 : score(v2);
+      v = v1 > -INFINITY ? s1 + (v2 > -INFINITY ? s2 : 0.f) : -INFINITY;
+    } else {
+      v = row_reduce<LG>(v1, max_op);
+    }
+    int before = 0;  // groups that come first
+    unrolled<1, G>([&](auto j) {
+      constexpr int CTRL = 0x120 + decltype(j)::value * LG;
+      const float o = rowf<CTRL>(v);
+      const int og = rowi<CTRL>(g);
+      before += o > v || (o == v && og < g) ? 1 : 0;
+    });
+    const bool keep = before < a.top_groups;
+    if (a.bias || a.top2) {
+      const float worst = row_reduce<16>(keep ? v : INFINITY, min_op);
+      const float next = row_reduce<16>(keep ? -INFINITY : v, max_op);
+      const float tol = 2.f * tol0 + 0x1.2p-22f * fabsf(worst);
+      unsure = next > -INFINITY && !(worst - next > tol);
+    }
+    // the kept groups, again over all lanes: lanes2 lanes for each of them
+    float* keys = s_key[tok];
+#pragma unroll
+    for (int p = 0; p < CH; ++p)
+      if (p < n) keys[e0 + p] = key[p];
+    uint32_t kept = (uint32_t)(__ballot(keep && sub == 0) >> (lane & 48)) & 0xffffu;
+    const int j = l16 / a.lanes2, sub2 = l16 - j * a.lanes2;
+    for (int i = 0; i + 1 < a.top_groups; ++i)
+      if (i < j) kept &= kept - 1;  // (unused lanes end with none, or with the last)
+    const int g2 = kept ? (__ffs((int)kept) - 1) / LG : 0, first2 = sub2 * a.chunk2;
+    int n2 = first2 >= a.gs ? 0 : a.gs - first2 < a.chunk2 ? a.gs - first2 : a.chunk2;
+    if (j >= a.top_groups) n2 = 0;
+    e0 = g2 * a.gs + first2;
+    __builtin_amdgcn_wave_barrier();
+    constexpr int H = CH / 2;
+    if (a.chunk2 <= H) {
+      float half[H];
+#pragma unroll
+      for (int p = 0; p < H; ++p) half[p] = p < n2 ? keys[e0 + p] : -INFINITY;
+      rank_experts<H, KC>(half, e0, a.k, lane, s_cand[tok], c, rank, total);
+    } else {
+#pragma unroll
+      for (int p = 0; p < CH; ++p) key[p] = p < n2 ? keys[e0 + p] : -INFINITY;
+      rank_experts<CH, KC>(key, e0, a.k, lane, s_cand[tok], c, rank, total);
+    }
+  } else {
+    rank_experts<CH, KC>(key, e0, a.k, lane, s_cand[tok], c, rank, total);
+  }
+  unsure |= total > 16 * KC;
+  if (a.bias) {  // keys are rounded scores: is one of the first k next to its follower?
+    float* sorted = s_sorted[tok];
+#pragma unroll
+    for (int i = 0; i < KC; ++i) sorted[rank[i]] = c[i].key;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < KC; ++i)
+      if (rank[i] < a.k && rank[i] + 1 < total) {
+        const float next = sorted[rank[i] + 1];
+        unsure |= !(c[i].key - next > tol0 + 0x1.2p-23f * fabsf(c[i].key));
+      }
+  }
+
+  // weights of the chosen: rank < k and an expert in the slot
+  bool in[KC];
+  float x[KC], w[KC], U = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < KC; ++i) {
+    in[i] = rank[i] < a.k && i * 16 + l16 < total;
+    x[i] = c[i].key;  // the logit itself, without a bias
+    if (a.bias)
+      x[i] = in[i] ? fminf(load_as_f32(a.logits, a.ldt, rr * a.E + c[i].id), FLT_MAX) : -INFINITY;
+    U = fmaxf(U, in[i] ? x[i] : -INFINITY);
+  }
+  U = row_reduce<16>(U, max_op);
+  if (a.sigmoid) U = fminf(U, 0.f);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < KC; ++i) {
+    if (a.renorm) {
+      w[i] = a.sigmoid && x[i] > 0.f ? 1.f / (1.f + expf(-x[i])) : expf(x[i] - U);
+      if (a.sigmoid && x[i] <= 0.f) w[i] = w[i] / (1.f + expf(x[i]));
+    } else {
+      w[i] = a.sigmoid ? 1.f / (1.f + expf(-x[i])) : expf(x[i] - m) / S;
+    }
+    if (!in[i]) w[i] = 0.f;
+    sum += w[i];
+  }
+  const float total_w = row_reduce<16>(sum, sum_op);
+  const bool padding = a.n_valid && row >= *a.n_valid;
+  const uint64_t again = __ballot(unsure && row < a.T && !padding);
+  if (row < a.T && !(again >> (lane & 48) & 0xffffu)) {
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      const bool use = in[i] && !padding;
+      const float v = a.renorm ? w[i] / total_w : w[i];
+      if (rank[i] < a.k) store_choice(a, row, rank[i], use ? c[i].id : -1, use ? v * a.scale : 0.f);
+    }
+  }
+#pragma unroll 1
+  for (int t = 0; t < 4; ++t)
+    if (again >> (16 * t) & 0xffffu)  // (the keys of the wave's tokens are not needed any more)
+      route_row<MAXC>(a, row0 + t, lane,
+                      reinterpret_cast<double*>(s_key[G > 1 ? (threadIdx.x >> 6) * 4 : 0]));
+}
+
+// The fast kernel's sizes: 1, 2, 4, 8 or 16 groups, at most 32 experts a lane and 24
+// choices (32 slots hold them with room for near ones).
+template <int CH, int G, int KC>
+int launch_tokens(const RouteArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((route_tokens_kernel<CH, G, KC, CH / 4 < 1 ? 1 : CH / 4>),
+                     dim3((unsigned)cdiv(a.T, 16)), dim3(256), 0, s, a);
+  return check_launch("route_tokens_kernel");
+}
+template <int CH, int G>
+int launch_slots(const RouteArgs& a, hipStream_t s) {
+  return a.k <= 10 ? launch_tokens<CH, G, 1>(a, s) : launch_tokens<CH, G, 2>(a, s);
+}
+template <int G>
+int launch_chunk(RouteArgs a, hipStream_t s) {
+  a.chunk = (int)cdiv(a.gs, 16 / G);
+  a.lanes2 = 16 / a.top_groups;
+  a.chunk2 = (int)cdiv(a.gs, a.lanes2);
+  a.vec = 0;
+  const int up = (a.chunk + 3) / 4 * 4;
+  if (a.gs % 4 == 0 && a.E % 4 == 0 && up <= 32 &&
+      (uintptr_t)a.logits % (4 * dtype_bytes(a.ldt)) == 0 &&
+      (!a.bias || (uintptr_t)a.bias % (4 * dtype_bytes(a.bdt)) == 0)) {
+    a.chunk = up;
+    a.vec = 1;
+  }
+  if (a.chunk <= 4) return launch_slots<4, G>(a, s);
+  if (a.chunk <= 8) return launch_slots<8, G>(a, s);
+  if (a.chunk <= 16) return launch_slots<16, G>(a, s);
+  return launch_slots<32, G>(a, s);
 }
 
 }  // namespace
@@ -287,8 +652,24 @@ extern "C" int exq_grouped_topk(const exq_route_problem* p, const void* logits, 
   a.top2 = p->group_score == EXQ_GROUP_TOP2;
   a.renorm = p->renormalize != 0;
   a.scale = p->scale;
-  const dim3 g((unsigned)cdiv(a.T, 4));
   const hipStream_t s = as_stream(stream);
+  if (a.k <= 24) {
+    // (with all groups kept they are one; their value is not asked for)
+    const int G = a.top_groups == a.G ? 1 : a.G;
+    RouteArgs f = a;
+    if (G == 1) {
+      f.G = f.top_groups = 1;
+      f.gs = a.E;
+    }
+    if (cdiv(f.gs, 16 / (G <= 16 ? G : 16)) <= 32) {
+      if (G == 1) return launch_chunk<1>(f, s);
+      if (G == 2) return launch_chunk<2>(f, s);
+      if (G == 4) return launch_chunk<4>(f, s);
+      if (G == 8) return launch_chunk<8>(f, s);
+      if (G == 16) return launch_chunk<16>(f, s);
+    }
+  }
+  const dim3 g((unsigned)cdiv(a.T, 4));
   if (a.E <= 256)
     hipLaunchKernelGGL(route_rows_kernel<4>, g, dim3(256), 0, s, a);
   else

@@ -240,13 +240,12 @@ def grouped_topk(gating_output: torch.Tensor, topk: int, renormalize: bool,
     ids = torch.empty(T, topk, dtype=ids_dtype, device=dev)
     wts = torch.empty(T, topk, dtype=weights_dtype, device=dev)
     code = _lib._TORCH_TO_CODE
-    p = _lib.RouteProblem(T, E, topk, num_expert_group, topk_group, code[g.dtype],
-                          0 if correction_bias is None else code[correction_bias.dtype],
-                          code[ids_dtype], code[weights_dtype], _SCORING[scoring_func],
-                          _GROUP_SCORE[group_score], 1 if renormalize else 0,
-                          routed_scaling_factor)
-    with _lib.on_device(dev):
-        _lib.check(_lib.lib().exq_grouped_topk(
-            p, g.data_ptr(), _lib.ptr(correction_bias), _lib.ptr(num_token_non_padded),
-            ids.data_ptr(), wts.data_ptr(), _lib.stream_handle(dev)), "grouped_topk")
+    p = _lib.route_problem(T, E, topk, num_expert_group, topk_group, code[g.dtype],
+                           0 if correction_bias is None else code[correction_bias.dtype],
+                           code[ids_dtype], code[weights_dtype], _SCORING[scoring_func],
+                           _GROUP_SCORE[group_score], 1 if renormalize else 0,
+                           float(routed_scaling_factor))
+    _lib.launch(_lib.lib().exq_grouped_topk,
+                (p, g.data_ptr(), _lib.ptr(correction_bias), _lib.ptr(num_token_non_padded),
+                 ids.data_ptr(), wts.data_ptr()), g.get_device(), "grouped_topk")
     return wts, ids

@@ -46,10 +46,11 @@ def _overlap(a: torch.Tensor, a_stride: int, b: torch.Tensor, b_stride: int) -> 
 
 
 def _call(x, weight, bias, activation, residual, out_dtype, out, n_out, gated, what):
-    if x.dim() != 2 or weight.dim() != 2:
+    shape, w_shape = x.shape, weight.shape
+    if len(shape) != 2 or len(w_shape) != 2:
         raise ValueError("x must be [T, K] and weight [N, K]")
-    T, K = x.shape
-    if weight.shape[1] != K or K < 1 or n_out < 1:
+    T, K = shape
+    if w_shape[1] != K or K < 1 or n_out < 1:
         raise ValueError(f"weight {tuple(weight.shape)} does not match x {tuple(x.shape)}")
     if x.dtype not in _ACT_DTYPES or weight.dtype != x.dtype:
         raise ValueError("x and weight must both be float16 or both bfloat16")
@@ -88,15 +89,14 @@ def _call(x, weight, bias, activation, residual, out_dtype, out, n_out, gated, w
     if out.dtype not in _FLOAT_DTYPES:
         raise ValueError("out_dtype must be float32, float16 or bfloat16")
     code = _lib._TORCH_TO_CODE
-    p = _lib.LinearProblem(T, K, n_out, ldx, ldw, ldr, ldo, code[x.dtype],
-                           0 if bias is None else code[bias.dtype],
-                           0 if residual is None else code[residual.dtype], code[out.dtype],
-                           _ACTIVATIONS[activation], gated)
-    with _lib.on_device(dev):
-        _lib.check(_lib.lib().exq_linear(
-            p, x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
-            None if residual is None else residual.data_ptr(), out.data_ptr(),
-            _lib.stream_handle(dev)), what)
+    p = _lib.linear_problem(T, K, n_out, ldx, ldw, ldr, ldo, code[x.dtype],
+                            0 if bias is None else code[bias.dtype],
+                            0 if residual is None else code[residual.dtype], code[out.dtype],
+                            _ACTIVATIONS[activation], gated)
+    _lib.launch(_lib.lib().exq_linear,
+                (p, x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
+                 None if residual is None else residual.data_ptr(), out.data_ptr()),
+                dev.index, what)
     return out
 
 

@@ -85,56 +85,67 @@ __device__ __forceinline__ void store_choice(const RouteArgs& a, int64_t row, in
   store_from_f32(a.wts, a.wdt, at, w);
 }
 
+// Weight of a chosen expert with logit x, not yet divided by the sum of a renormalised
+// row: s(x), times e^-U where it will be, U = the largest of the chosen x (sigmoid: at
+// most 0), so that scores which all underflow still have their ratio.
+__device__ __forceinline__ float choice_weight(const RouteArgs& a, float x, float U, float m,
+                                               float S) {
+  const float d = a.renorm ? U : a.sigmoid ? 0.f : m;
+  const float e = expf(a.sigmoid && x > 0.f ? -x : x - d);
+  if (!a.sigmoid) return a.renorm ? e : e / S;
+  return x > 0.f ? 1.f / (1.f + e) : e / (1.f + expf(x));
+}
+
 // One token, by one wave, ranked in 64 bits: neither an expert nor a group is
 // decided by the rounding of a score.  Lane l holds experts l + 64 c; `mem` is E doubles
-// of the wave's own LDS, used where groups are chosen.  The weights are the chosen
-// scores: exp(u - U) / sum with u = l (softmax) or log(sigmoid(l)) = min(l, 0) -
-// log1p(exp(-|l|)), and U the largest chosen u where they are renormalised, so
-// that scores which all underflow still have their ratio.
+// of the wave's own LDS.  The loops over c stay rolled where they hold an exponential:
+// as the rare part of route_tokens_kernel this runs from a cold instruction cache.
 template <int MAXC>
 __device__ void route_row(const RouteArgs& a, int64_t row, int lane, double* mem) {
-  double r[MAXC];  // rank values, -inf where an expert is masked or taken
-  float lg[MAXC];
+  float b[MAXC];
   float m = -FLT_MAX;
 #pragma unroll
-  for (int c = 0; c < MAXC; ++c) {
+  for (int c = 0; c < MAXC; ++c) {  // mem: the logits, -inf where the expert is masked
     const int e = lane + 64 * c;
-    lg[c] = -INFINITY;
+    b[c] = 0.f;
     if (e < a.E) {
       const float l = load_as_f32(a.logits, a.ldt, row * a.E + e);
-      const float b = a.bias ? load_as_f32(a.bias, a.bdt, e) : 0.f;
-      if (l > -INFINITY && b > -INFINITY) lg[c] = fminf(l, FLT_MAX);
+      if (a.bias) b[c] = load_as_f32(a.bias, a.bdt, e);
+      const float x = l > -INFINITY && b[c] > -INFINITY ? fminf(l, FLT_MAX) : -INFINITY;
+      m = fmaxf(m, x);
+      mem[e] = x;
     }
-    m = fmaxf(m, lg[c]);
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-  const bool by_sum = a.top_groups < a.G && a.top2;
-  double S = 0.0;
+  double S = 1.0;
   if (!a.sigmoid) {
 #pragma unroll
-    for (int c = 0; c < MAXC; ++c) {
-      r[c] = lg[c] > -INFINITY ? exp((double)lg[c] - (double)m) : 0.0;
-      S += r[c];
-    }
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    S = 0.0;
+#pragma unroll 1
+    for (int e = lane; e < a.E; e += 64) S += exp(mem[e] - (double)m);  // (0 for -inf)
     S = wave_sum64(S);
-  } else if (a.bias || by_sum) {
-#pragma unroll
-    for (int c = 0; c < MAXC; ++c) r[c] = 1.0 / (1.0 + exp(-(double)lg[c]));
   }
+  auto score = [&](double l) {
+    const double e = exp(a.sigmoid ? -l : l - (double)m);
+    return a.sigmoid ? 1.0 / (1.0 + e) : e / S;
+  };
+  if (a.bias) {
+#pragma unroll 1
+    for (int e = lane; e < a.E; e += 64) {
+      const double l = mem[e];
+      mem[e] = l > -INFINITY ? score(l) : l;
+    }
 #pragma unroll
-  for (int c = 0; c < MAXC; ++c) {
-    const int e = lane + 64 * c;
-    const bool there = lg[c] > -INFINITY;
-    const double s = a.sigmoid ? r[c] : r[c] / S;
-    if (by_sum && !a.bias && e < a.E) mem[e] = there ? s : -INFINITY;
-    r[c] = !there ? -INFINITY : a.bias ? s + (double)load_as_f32(a.bias, a.bdt, e) : (double)lg[c];
-    if (a.top_groups < a.G && !(by_sum && !a.bias) && e < a.E) mem[e] = r[c];
+    for (int c = 0; c < MAXC; ++c) {  // (a masked expert's bias may be infinite or NaN)
+      const int e = lane + 64 * c;
+      if (e < a.E && mem[e] > -INFINITY) mem[e] += (double)b[c];
+    }
   }
+  __builtin_amdgcn_wave_barrier();  // (the wave's own LDS, in order)
 
+  uint64_t keep = ~0ull;
   if (a.top_groups < a.G) {
     // lane g: the value of group g, and how many groups come before it
-    __builtin_amdgcn_wave_barrier();
     double v1 = -INFINITY, v2 = -INFINITY;
     if (lane < a.G) {
       auto take = [&](double x) {
@@ -143,32 +154,43 @@ __device__ void route_row(const RouteArgs& a, int64_t row, int lane, double* mem
       };
       const double* at = mem + lane * a.gs;
       int i = 0;
-      for (; i + 8 <= a.gs; i += 8) {  // (eight reads in flight)
-        double x[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) x[q] = at[i + q];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) take(x[q]);
+      for (; i + 4 <= a.gs; i += 4) {  // (four reads in flight)
+        const double x0 = at[i], x1 = at[i + 1], x2 = at[i + 2], x3 = at[i + 3];
+        take(x0);
+        take(x1);
+        take(x2);
+        take(x3);
       }
       for (; i < a.gs; ++i) take(at[i]);
     }
-    if (a.top2 && v2 > -INFINITY) v1 = v1 + v2;
+    if (a.top2 && v1 > -INFINITY) {
+      if (!a.bias) {  // the sum is of scores, not of the logits that rank them
+#pragma unroll 1
+        for (int q = 0; q < 2; ++q) {
+          const double t = v1;
+          v1 = v2;
+          v2 = t > -INFINITY ? score(t) : t;
+        }
+        // (twice swapped: v1 and v2 are the scores of what they were)
+      }
+      if (v2 > -INFINITY) v1 += v2;
+    }
     int before = 0;
-#pragma unroll 4
     for (int g = 0; g < a.G; ++g) {
       const double o = __shfl(v1, g, 64);
       before += o > v1 || (o == v1 && g < lane) ? 1 : 0;
     }
-    const uint64_t keep = __ballot(lane < a.G && before < a.top_groups);
+    keep = __ballot(lane < a.G && before < a.top_groups);
+  }
+  double r[MAXC];  // rank values, -inf where an expert is masked, out of the groups or taken
 #pragma unroll
-    for (int c = 0; c < MAXC; ++c) {
-      const int e = lane + 64 * c;
-      if (e < a.E && !(keep >> (e / a.gs) & 1u)) r[c] = -INFINITY;
-    }
+  for (int c = 0; c < MAXC; ++c) {
+    const int e = lane + 64 * c;
+    r[c] = -INFINITY;
+    if (e < a.E && (a.top_groups >= a.G || keep >> (e / a.gs) & 1u)) r[c] = mem[e];
   }
 
   int my_id = -1;
-  float my_l = -INFINITY;
   for (int j = 0; j < a.k; ++j) {
     double bv = -INFINITY;
     int be = 0;
@@ -185,33 +207,25 @@ __device__ void route_row(const RouteArgs& a, int64_t row, int lane, double* mem
                       ? __builtin_amdgcn_readlane(
                             be, __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)at) - 1))
                       : (int)wave_min(bv == M ? (uint32_t)be : 0xffffffffu);
-    float l = 0.f;
 #pragma unroll
     for (int c = 0; c < MAXC; ++c)
-      if (lane + 64 * c == e) {
-        r[c] = -INFINITY;
-        l = lg[c];
-      }
-    l = __shfl(l, e & 63, 64);
-    if (lane == j) {
-      my_id = e;
-      my_l = l;
-    }
+      if (lane + 64 * c == e) r[c] = -INFINITY;
+    if (lane == j) my_id = e;
   }
-  double w = 0.0;
-  if (my_id >= 0) {
-    w = my_l;
-    if (a.sigmoid) w = fmin(w, 0.0) - log1p(exp(-fabs(w)));
-  }
+  const float x =
+      my_id >= 0 ? fminf(load_as_f32(a.logits, a.ldt, row * a.E + my_id), FLT_MAX) : -INFINITY;
+  float U = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) U = fmaxf(U, __shfl_xor(U, d, 64));
+  if (a.sigmoid) U = fminf(U, 0.f);
+  float w = my_id >= 0 ? choice_weight(a, x, U, m, (float)S) : 0.f;
   if (a.renorm) {
-    const double U = wave_max64(my_id >= 0 ? w : -INFINITY);
-    w = my_id >= 0 ? exp(w - U) : 0.0;
-    const double sum = wave_sum64(w);
-    w = my_id >= 0 ? w / sum : 0.0;
-  } else if (my_id >= 0) {
-    w = a.sigmoid ? exp(w) : exp(w - (double)m) / S;
+    float sum = w;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    w = my_id >= 0 ? w / sum : 0.f;
   }
-  if (lane < a.k) store_choice(a, row, lane, my_id, (float)(w * (double)a.scale));
+  if (lane < a.k) store_choice(a, row, lane, my_id, w * a.scale);
 }
 
 template <int MAXC>
@@ -365,7 +379,7 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
   constexpr int KEYS = 16 * CH + 4;  // floats of a token's keys in LDS
   __shared__ Candidate s_cand[16][16 * KC + 1];
   __shared__ float s_sorted[16][16 * KC + 1];
-  __shared__ __align__(16) float s_key[G > 1 ? 16 : 1][G > 1 ? KEYS : 4];
+  __shared__ __align__(16) float s_key[16][KEYS];  // (route_row: 16 CH doubles a wave)
   const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int tok = threadIdx.x >> 4;   // token of the work-group
   const int row0 = blockIdx.x * 16 + (threadIdx.x >> 6) * 4;  // first row of the wave
@@ -540,12 +554,7 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < KC; ++i) {
-    if (a.renorm) {
-      w[i] = a.sigmoid && x[i] > 0.f ? 1.f / (1.f + expf(-x[i])) : expf(x[i] - U);
-      if (a.sigmoid && x[i] <= 0.f) w[i] = w[i] / (1.f + expf(x[i]));
-    } else {
-      w[i] = a.sigmoid ? 1.f / (1.f + expf(-x[i])) : expf(x[i] - m) / S;
-    }
+    w[i] = choice_weight(a, x[i], U, m, S);
     if (!in[i]) w[i] = 0.f;
     sum += w[i];
   }
@@ -564,7 +573,7 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
   for (int t = 0; t < 4; ++t)
     if (again >> (16 * t) & 0xffffu)  // (the keys of the wave's tokens are not needed any more)
       route_row<MAXC>(a, row0 + t, lane,
-                      reinterpret_cast<double*>(s_key[G > 1 ? (threadIdx.x >> 6) * 4 : 0]));
+                      reinterpret_cast<double*>(s_key[(threadIdx.x >> 6) * 4]));
 }
 
 // The fast kernel's sizes: 1, 2, 4, 8 or 16 groups, at most 32 experts a lane and 24

@@ -59,90 +59,6 @@ __device__ __forceinline__ void activate_run(float (&v)[CNT], int act) {
   }
 }
 
-// One output (token m, column n) of the product `y` (gated: `y` gate and `u` up).
-template <bool GATED>
-__device__ __forceinline__ float finish(const LinArgs& a, int64_t m, int64_t n, float y, float u) {
-  if (a.bias) {
-    y += load_as_f32(a.bias, a.bdt, n);
-    if (GATED) u += load_as_f32(a.bias, a.bdt, a.N + n);
-  }
-  float v[1] = {y};
-  activate_run<1>(v, a.act);
-  y = v[0];
-  if (GATED) return y * u;
-  if (a.res) y += load_as_f32(a.res, a.rdt, m * a.ldr + n);
-  return y;
-}
-
-// ---- any layout -------------------------------------------------------------
-// Eight consecutive elements [k, k + 8) of a row as they lie, at any 2-byte
-// alignment; zeros from K on.
-struct __attribute__((packed, aligned(2))) Chunk {
-  uint32_t d[4];
-};
-__device__ __forceinline__ uint4 load_chunk(const uint16_t* row, int64_t k, int64_t K) {
-  if (k + 8 <= K) {
-    const Chunk c = *reinterpret_cast<const Chunk*>(row + k);
-    return uint4{c.d[0], c.d[1], c.d[2], c.d[3]};
-  }
-  uint32_t d[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (k + j < K) d[j >> 1] |= (uint32_t)row[k + j] << ((j & 1) * 16);
-  return uint4{d[0], d[1], d[2], d[3]};
-}
-
-// 64 tokens x 64 weight rows (gated: 32 gate and the 32 matching up rows) by four
-// waves, each 16 tokens x all weight rows; 32 k at a time through registers into
-// LDS.  For rows that are not 16-byte aligned or K % 8 != 0.
-constexpr int GB = 64, GK = 32, GLD = GK + 8;
-
-template <bool BF, bool GATED>
-__global__ void __launch_bounds__(256) linear_any_kernel(LinArgs a) {
-  __shared__ __align__(16) uint16_t sx[GB * GLD];
-  __shared__ __align__(16) uint16_t sw[GB * GLD];
-  constexpr int BN = GATED ? GB / 2 : GB;  // output columns of the tile
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int r16 = lane & 15, q = lane >> 4;
-  const int64_t m0 = (int64_t)blockIdx.x * GB, n0 = (int64_t)blockIdx.y * BN;
-  const int row = tid >> 2, ch = (tid & 3) * 8;
-  const int64_t xr = m0 + row;
-  const int64_t wn = n0 + (GATED ? row % BN : row);
-  const bool xin = xr < a.T, win = wn < a.N;
-  const uint16_t* xp = a.x + (xin ? xr : 0) * a.ldx;
-  const uint16_t* wp = a.w + ((win ? wn : 0) + (GATED && row >= BN ? a.N : 0)) * a.ldw;
-  const uint4 zero = uint4{0u, 0u, 0u, 0u};
-  f32x4_t acc[4] = {};
-  uint4 vx = xin ? load_chunk(xp, ch, a.K) : zero;
-  uint4 vw = win ? load_chunk(wp, ch, a.K) : zero;
-  for (int64_t k0 = 0; k0 < a.K; k0 += GK) {
-    __syncthreads();
-    *reinterpret_cast<uint4*>(sx + row * GLD + ch) = vx;
-    *reinterpret_cast<uint4*>(sw + row * GLD + ch) = vw;
-    __syncthreads();
-    if (k0 + GK < a.K) {
-      vx = xin ? load_chunk(xp, k0 + GK + ch, a.K) : zero;
-      vw = win ? load_chunk(wp, k0 + GK + ch, a.K) : zero;
-    }
-    const uint4 b = *reinterpret_cast<const uint4*>(sx + (wave * 16 + r16) * GLD + q * 8);
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-      acc[t] = mfma<BF>(*reinterpret_cast<const uint4*>(sw + (t * 16 + r16) * GLD + q * 8), b,
-                        acc[t]);
-  }
-  const int64_t m = m0 + wave * 16 + r16;
-  if (m >= a.T) return;
-#pragma unroll
-  for (int t = 0; t < (GATED ? 2 : 4); ++t)
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int64_t n = n0 + t * 16 + q * 4 + v;
-      if (n < a.N)
-        store_from_f32(a.out, a.odt, m * a.ldo + n,
-                       finish<GATED>(a, m, n, acc[t][v], GATED ? acc[(t + 2) & 3][v] : 0.f));
-    }
-}
-
 // ---- aligned rows: copies straight into LDS ----------------------------------
 // 16 bytes per lane from buffer `r` at byte offset voff + soff into LDS at
 // lds + 16 * lane; `lds` and `soff` are wave-uniform.  A voff past the resource
@@ -317,6 +233,39 @@ __device__ __forceinline__ bool unit_of(int bid, int nm, int nn, int& mt, int& n
   return true;
 }
 
+// The sums of W waves over their parts of the contraction, joined through LDS in wave
+// order, and their epilogue: 16 MT tokens x 16 NT weight rows.
+template <bool GATED, int MT, int NT, int W>
+__device__ __forceinline__ void join_waves(const LinArgs& a, float4* red,
+                                           const f32x4_t (&acc)[MT][NT], int64_t m0, int64_t n0,
+                                           int wave, int lane) {
+  constexpr int TILES = GATED ? NT / 2 : NT;
+#pragma unroll
+  for (int u = 0; u < MT; ++u)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      red[((wave * MT + u) * NT + t) * 64 + lane] =
+          float4{acc[u][t][0], acc[u][t][1], acc[u][t][2], acc[u][t][3]};
+  __syncthreads();
+  for (int u = wave; u < MT; u += W) {
+    const int64_t m = m0 + u * 16 + (lane & 15), n = n0 + (lane >> 4) * 4 * TILES;
+    float y[4 * TILES], up[4 * TILES], res[4 * TILES];
+    if constexpr (!GATED) fetch_residual<4 * TILES>(a, m, n, res);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float4 s = red[(u * NT + t) * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < W; ++w) {
+        const float4 p = red[((w * MT + u) * NT + t) * 64 + lane];
+        s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
+      }
+      float* o = GATED && t >= TILES ? up + (t - TILES) * 4 : y + (t % TILES) * 4;
+      o[0] = s.x; o[1] = s.y; o[2] = s.z; o[3] = s.w;
+    }
+    finish_run<4 * TILES, GATED>(a, m, n, y, up, res);
+  }
+}
+
 // ---- few tokens: a stream of weights -------------------------------------------
 // 16 MT tokens x 16 NT weight rows by W waves that split the contraction: wave w
 // takes the 64-k steps w, w + W, ... of all the tile's rows through an LDS ring of
@@ -399,30 +348,7 @@ __global__ void __launch_bounds__(64 * W) linear_stream_kernel(LinArgs a, int nm
   }
   wait_vm<0>();
   __syncthreads();
-  float4* red = reinterpret_cast<float4*>(lds);
-#pragma unroll
-  for (int u = 0; u < MT; ++u)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-      red[((wave * MT + u) * NT + t) * 64 + lane] =
-          float4{acc[u][t][0], acc[u][t][1], acc[u][t][2], acc[u][t][3]};
-  __syncthreads();
-  for (int u = wave; u < MT; u += W) {
-    float y[4 * TILES], up[4 * TILES], res[4 * TILES];
-    if constexpr (!GATED) fetch_residual<4 * TILES>(a, m0 + u * 16 + r16, n0 + q * 4 * TILES, res);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float4 s = red[(u * NT + t) * 64 + lane];
-#pragma unroll
-      for (int w = 1; w < W; ++w) {
-        const float4 p = red[((w * MT + u) * NT + t) * 64 + lane];
-        s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
-      }
-      float* o = GATED && t >= TILES ? up + (t - TILES) * 4 : y + (t % TILES) * 4;
-      o[0] = s.x; o[1] = s.y; o[2] = s.z; o[3] = s.w;
-    }
-    finish_run<4 * TILES, GATED>(a, m0 + u * 16 + r16, n0 + q * 4 * TILES, y, up, res);
-  }
+  join_waves<GATED, MT, NT, W>(a, reinterpret_cast<float4*>(lds), acc, m0, n0, wave, lane);
 }
 
 // ---- many tokens: tiles ------------------------------------------------------------
@@ -472,6 +398,26 @@ __device__ __forceinline__ void finish_wave(const LinArgs& a, const float* sums,
       }
       finish_run<8, GATED>(a, m0 + m, n0 + c * 8, y, up, r[b]);
     }
+  }
+}
+
+// A wave's sums, through memory of its own in LDS 32 tokens at a time.
+template <bool GATED, int MT, int NT>
+__device__ __forceinline__ void store_sums(const LinArgs& a, float* sums,
+                                           const f32x16_t (&acc)[MT][NT], int64_t m0, int64_t n0,
+                                           int lane) {
+  const int r32 = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int u = 0; u < MT; ++u) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int v = 0; v < 16; v += 4)
+        *reinterpret_cast<float4*>(sums + r32 * pitch<NT>() + t * 32 + 2 * v + 4 * h) =
+            float4{acc[u][t][v], acc[u][t][v + 1], acc[u][t][v + 2], acc[u][t][v + 3]};
+    __builtin_amdgcn_sched_barrier(0);  // (a few sums at a time leave the accumulators)
+    finish_wave<GATED, NT>(a, sums, m0 + u * 32, n0, lane);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -649,20 +595,138 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(LinArgs a, in
   }
   wait_vm<0>();
   __syncthreads();
-  // the sums go through LDS 32 tokens at a time, in memory of the wave's own
-  float* sums = reinterpret_cast<float*>(lds) + wave * 32 * pitch<NT>();
-#pragma unroll
-  for (int u = 0; u < MT; ++u) {
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int v = 0; v < 16; v += 4)
-        *reinterpret_cast<float4*>(sums + r32 * pitch<NT>() + t * 32 + 2 * v + 4 * h) =
-            float4{acc[u][t][v], acc[u][t][v + 1], acc[u][t][v + 2], acc[u][t][v + 3]};
-    __builtin_amdgcn_sched_barrier(0);  // (a few sums at a time leave the accumulators)
-    finish_wave<GATED, NT>(a, sums, m0 + (wm * MT + u) * 32, n0 + wn * WC, lane);
-    __builtin_amdgcn_sched_barrier(0);
+  store_sums<GATED, MT, NT>(a, reinterpret_cast<float*>(lds) + wave * 32 * pitch<NT>(), acc,
+                            m0 + wm * MT * 32, n0 + wn * WC, lane);
+}
+
+// ---- any layout --------------------------------------------------------------------
+// Rows that are not 16-byte aligned, or K % 8 != 0: no copies into LDS, but unaligned
+// 16-byte loads.  Eight consecutive elements [k, k + 8) of a row, zeros from K on.
+struct __attribute__((packed, aligned(2))) Chunk {
+  uint32_t d[4];
+};
+__device__ __forceinline__ uint4 load_chunk(const uint16_t* row, int k, int K) {
+  if (k + 8 <= K) {
+    const Chunk c = *reinterpret_cast<const Chunk*>(row + k);
+    return uint4{c.d[0], c.d[1], c.d[2], c.d[3]};
   }
+  uint32_t d[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (k + j < K) d[j >> 1] |= (uint32_t)row[k + j] << ((j & 1) * 16);
+  return uint4{d[0], d[1], d[2], d[3]};
+}
+
+// Few tokens: as linear_stream_kernel, the matrix operands straight from memory.
+// Wave w takes the 32-k steps w, w + W, ..., U of them in flight.
+template <bool BF, bool GATED, int MT, int NT, int W, int U>
+__global__ void __launch_bounds__(64 * W) linear_stream_any_kernel(LinArgs a, int nm, int nn) {
+  constexpr int TILES = GATED ? NT / 2 : NT;
+  __shared__ __align__(16) float4 red[W * MT * NT * 64];
+  int mb, nb;
+  if (!unit_of<4>(blockIdx.x, nm, nn, mb, nb)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, q = lane >> 4;
+  const int64_t m0 = (int64_t)mb * MT * 16, n0 = (int64_t)nb * TILES * 16;
+  const int K = (int)a.K;
+  // (rows past the last repeat it: what they give is not stored)
+  const uint16_t *xp[MT], *wp[NT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int64_t m = m0 + t * 16 + r16;
+    xp[t] = a.x + (m < a.T ? m : a.T - 1) * a.ldx + q * 8;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t n = n0 + run_col<TILES>(t % TILES, r16);
+    wp[t] = a.w + ((n < a.N ? n : a.N - 1) + (t >= TILES ? a.N : 0)) * a.ldw + q * 8;
+  }
+  f32x4_t acc[MT][NT] = {};
+  for (int k0 = wave * 32; k0 < K; k0 += 32 * W * U) {
+    uint4 x[U][MT], w[U][NT];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int k = k0 + i * 32 * W, left = K - q * 8;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) w[i][t] = load_chunk(wp[t], k, left);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) x[i][t] = load_chunk(xp[t], k, left);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) acc[u][t] = mfma<BF>(w[i][t], x[i][u], acc[u][t]);
+  }
+  join_waves<GATED, MT, NT, W>(a, red, acc, m0, n0, wave, lane);
+}
+
+// Many tokens: 32 MT WM x 32 NT WN tiles as in linear_tile_kernel, a block's rows
+// through registers into one of two LDS stages.
+template <bool BF, bool GATED, int WM, int WN, int MT, int NT>
+__global__ void __launch_bounds__(64 * WM * WN) linear_tile_any_kernel(LinArgs a, int nm, int nn) {
+  constexpr int W = WM * WN, THREADS = 64 * W;
+  constexpr int BM = 32 * MT * WM, BR = 32 * NT * WN;
+  constexpr int WC = (GATED ? 16 : 32) * NT;
+  constexpr int KB = 64, STAGE = (BM + BR) * 2 * KB;
+  constexpr int D = (BM + BR) * 8 / THREADS;       // 16-byte chunks of a thread and block
+  constexpr int SUMS = W * 32 * pitch<NT>() * 4;
+  constexpr int LDS = 2 * STAGE > SUMS ? 2 * STAGE : SUMS;
+  __shared__ __align__(1024) unsigned char lds[LDS];
+  int mb, nb;
+  if (!unit_of<8>(blockIdx.x, nm, nn, mb, nb)) return;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, h = lane >> 5;
+  const int wm = wave / WN, wn = wave % WN;
+  const int64_t m0 = (int64_t)mb * BM, n0 = (int64_t)nb * WC * WN;
+  const int K = (int)a.K;
+  const int ch = tid & 7;                          // chunk of the thread's rows
+  const uint16_t* rows[D];                         // (rows past the last repeat it)
+  int at[D];
+#pragma unroll
+  for (int j = 0; j < D; ++j) {
+    const int r = j * (THREADS / 8) + (tid >> 3);
+    const int rw = r - BM, c = GATED ? (rw >> 5) * 16 + (rw & 15) : rw;
+    const int64_t m = m0 + r, n = n0 + c;
+    rows[j] = r < BM ? a.x + (m < a.T ? m : a.T - 1) * a.ldx
+                     : a.w + ((n < a.N ? n : a.N - 1) + (GATED && (rw >> 4) & 1 ? a.N : 0)) * a.ldw;
+    at[j] = r * 128 + (ch ^ swz(r)) * 16;
+  }
+  f32x16_t acc[MT][NT] = {};
+  const int xo = (wm * MT * 32 + r32) * 128, wo = BM * 128 + (wn * NT * 32 + r32) * 128;
+  const int sw = swz(r32) * 16, hb = h * 16;
+  uint4 v[D];
+#pragma unroll
+  for (int j = 0; j < D; ++j) v[j] = load_chunk(rows[j], ch * 8, K);
+  const int nk = (K + KB - 1) / KB;
+  for (int kb = 0; kb < nk; ++kb) {
+    unsigned char* stage = lds + (kb & 1) * STAGE;
+#pragma unroll
+    for (int j = 0; j < D; ++j) *reinterpret_cast<uint4*>(stage + at[j]) = v[j];
+    __syncthreads();  // (the stage written next was read before this)
+    if (kb + 1 < nk) {
+#pragma unroll
+      for (int j = 0; j < D; ++j) v[j] = load_chunk(rows[j], (kb + 1) * KB + ch * 8, K);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const unsigned char* p = stage + ((s * 32 + hb) ^ sw);
+      uint4 fx[MT], fw[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) fw[t] = *reinterpret_cast<const uint4*>(p + wo + t * 4096);
+#pragma unroll
+      for (int u = 0; u < MT; ++u) fx[u] = *reinterpret_cast<const uint4*>(p + xo + u * 4096);
+#pragma unroll
+      for (int u = 0; u < MT; ++u)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[u][t] = mfma32<BF>(fw[t], fx[u], acc[u][t]);
+    }
+  }
+  __syncthreads();
+  store_sums<GATED, MT, NT>(a, reinterpret_cast<float*>(lds) + wave * 32 * pitch<NT>(), acc,
+                            m0 + wm * MT * 32, n0 + wn * WC, lane);
 }
 
 // Whether `rows` rows of stride ld fit one buffer resource.
@@ -670,21 +734,41 @@ inline bool span_fits(int64_t rows, int64_t ld, int64_t K) {
   return ((rows - 1) * ld + K + 64) * 2 < kSpan;
 }
 
+// Work-groups of a grid of nm x nn tiles, a multiple of the XCDs; 0: more than a launch
+// takes.
+int64_t tile_grid(int64_t nm, int64_t nn, int threads) {
+  const int64_t n = cdiv(nm * nn, 8) * 8;
+  return n * threads < ((int64_t)1 << 32) ? n : 0;
+}
+template <typename Kernel>
+int launch_tiles(Kernel kernel, const LinArgs& a, int64_t tokens, int64_t cols, int threads,
+                 hipStream_t s) {
+  const int64_t nm = cdiv(a.T, tokens), nn = cdiv(a.N, cols), grid = tile_grid(nm, nn, threads);
+  EXQ_REQUIRE_SUPPORTED(grid > 0, "exq_linear: T=%lld x N=%lld is too large", (long long)a.T,
+                        (long long)a.N);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3((unsigned)threads), 0, s, a, (int)nm,
+                     (int)nn);
+  return check_launch("linear kernel");
+}
 template <bool BF, bool GATED, int MT, int NT, int W, int NST>
 int launch_stream(const LinArgs& a, hipStream_t s) {
-  const int nm = (int)cdiv(a.T, MT * 16), nn = (int)cdiv(a.N, (GATED ? NT / 2 : NT) * 16);
-  hipLaunchKernelGGL((linear_stream_kernel<BF, GATED, MT, NT, W, NST>),
-                     dim3((unsigned)(cdiv((int64_t)nm * nn, 8) * 8)), dim3(64 * W), 0, s, a, nm,
-                     nn);
-  return check_launch("linear_stream_kernel");
+  return launch_tiles(linear_stream_kernel<BF, GATED, MT, NT, W, NST>, a, 16 * MT,
+                      (GATED ? 8 : 16) * NT, 64 * W, s);
+}
+template <bool BF, bool GATED, int MT, int NT, int W, int U>
+int launch_stream_any(const LinArgs& a, hipStream_t s) {
+  return launch_tiles(linear_stream_any_kernel<BF, GATED, MT, NT, W, U>, a, 16 * MT,
+                      (GATED ? 8 : 16) * NT, 64 * W, s);
 }
 template <bool BF, bool GATED, int WM, int WN, int MT, int NT, int NST, int PF, bool AHEAD>
 int launch_tile(const LinArgs& a, hipStream_t s) {
-  const int nm = (int)cdiv(a.T, 32 * MT * WM), nn = (int)cdiv(a.N, (GATED ? 16 : 32) * NT * WN);
-  hipLaunchKernelGGL((linear_tile_kernel<BF, GATED, WM, WN, MT, NT, NST, PF, AHEAD>),
-                     dim3((unsigned)(cdiv((int64_t)nm * nn, 8) * 8)), dim3(64 * WM * WN), 0, s, a,
-                     nm, nn);
-  return check_launch("linear_tile_kernel");
+  return launch_tiles(linear_tile_kernel<BF, GATED, WM, WN, MT, NT, NST, PF, AHEAD>, a,
+                      32 * MT * WM, (GATED ? 16 : 32) * NT * WN, 64 * WM * WN, s);
+}
+template <bool BF, bool GATED, int WM, int WN, int MT, int NT>
+int launch_tile_any(const LinArgs& a, hipStream_t s) {
+  return launch_tiles(linear_tile_any_kernel<BF, GATED, WM, WN, MT, NT>, a, 32 * MT * WM,
+                      (GATED ? 16 : 32) * NT * WN, 64 * WM * WN, s);
 }
 
 // Which kernel: the one with the least rounds x time of a round, where a round is as
@@ -727,7 +811,7 @@ template <bool BF, bool GATED>
 int launch_linear(const LinArgs& a, hipStream_t s) {
   const bool aligned = (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0 && a.ldx % 8 == 0 &&
                        a.ldw % 8 == 0 && a.K % 8 == 0 && span_fits(256, a.ldx, a.K) &&
-                       span_fits(256, a.ldw, a.K) && cdiv(a.T, 16) * cdiv(a.N, 16) < (1 << 30);
+                       span_fits(256, a.ldw, a.K);
   if (aligned) {
     switch (pick_shape(a.T, a.N * (GATED ? 2 : 1))) {
       case 0: return launch_stream<BF, GATED, 1, 2, 8, 3>(a, s);
@@ -741,10 +825,12 @@ int launch_linear(const LinArgs& a, hipStream_t s) {
       default: return launch_tile<BF, GATED, 2, 2, 4, 4, 2, 4, false>(a, s);
     }
   }
-  const int64_t bn = GATED ? GB / 2 : GB;
-  const dim3 g((unsigned)cdiv(a.T, GB), (unsigned)cdiv(a.N, bn));
-  hipLaunchKernelGGL((linear_any_kernel<BF, GATED>), g, dim3(256), 0, s, a);
-  return check_launch("linear_any_kernel");
+  const int64_t rows = a.N * (GATED ? 2 : 1);
+  if (a.T <= 16) return launch_stream_any<BF, GATED, 1, 2, 8, 4>(a, s);
+  if (cdiv(a.T, 32) * cdiv(rows, 32) <= 2 * kCus)
+    return launch_stream_any<BF, GATED, 2, 2, 8, 2>(a, s);
+  if (cdiv(a.T, 128) * cdiv(rows, 128) <= kCus) return launch_tile_any<BF, GATED, 2, 2, 1, 1>(a, s);
+  return launch_tile_any<BF, GATED, 2, 2, 2, 2>(a, s);
 }
 
 }  // namespace

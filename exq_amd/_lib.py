@@ -156,18 +156,6 @@ def stream_handle(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if i is None else i)
 
 
-@functools.lru_cache(maxsize=4096)
-def route_problem(*fields) -> RouteProblem:
-    """The problem of a grouped_topk call, which the library only reads."""
-    return RouteProblem(*fields)
-
-
-@functools.lru_cache(maxsize=4096)
-def linear_problem(*fields) -> LinearProblem:
-    """The problem of a fused_linear call, which the library only reads."""
-    return LinearProblem(*fields)
-
-
 def launch(entry, args: tuple, index: int, what: str) -> None:
     """``entry(*args, stream)`` on the current stream of device ``index``, which is made
     the current device for the call where it is not."""

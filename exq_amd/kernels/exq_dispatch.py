@@ -9,6 +9,8 @@ points the reference pipeline calls (``moe_align_block_size`` and
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
@@ -178,6 +180,41 @@ _GROUP_SCORE = {"max": 0, "top2": 1}
 _FLOAT_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
+@functools.lru_cache(maxsize=4096)
+def _route_problem(shape, dtype, bias, topk, renormalize, num_expert_group, topk_group,
+                   scoring_func, group_score, scale, ids_dtype, weights_dtype):
+    """The checked problem of a grouped_topk call, a function of its layouts and options
+    alone (so they are checked once; the library only reads the problem)."""
+    if len(shape) != 2:
+        raise ValueError("gating_output must be [T, E]")
+    if dtype not in _FLOAT_DTYPES:
+        raise ValueError("gating_output must be float32, float16 or bfloat16")
+    T, E = shape
+    if not 1 <= E <= 1024:
+        raise ValueError(f"E={E} experts is not in [1, 1024]")
+    if not 1 <= num_expert_group <= 64 or E % num_expert_group:
+        raise ValueError(f"num_expert_group={num_expert_group} must divide E={E} and be at most 64")
+    if not 1 <= topk_group <= num_expert_group:
+        raise ValueError(f"topk_group={topk_group} must be in [1, num_expert_group]")
+    if not 1 <= topk <= min(64, E // num_expert_group * topk_group):
+        raise ValueError(f"topk={topk} must be in [1, 64] and fit the experts of topk_group groups")
+    if scoring_func not in _SCORING:
+        raise ValueError(f"unsupported scoring_func {scoring_func!r}")
+    if group_score is None:
+        group_score = "max" if bias is None else "top2"
+    if group_score not in _GROUP_SCORE:
+        raise ValueError(f"unsupported group_score {group_score!r}")
+    if ids_dtype not in (torch.int32, torch.int64) or weights_dtype not in _FLOAT_DTYPES:
+        raise ValueError("ids must be int32 or int64, weights float32, float16 or bfloat16")
+    if bias is not None and (bias[1] not in _FLOAT_DTYPES or tuple(bias[0]) != (E,)):
+        raise ValueError(f"correction_bias must be [{E}], float32, float16 or bfloat16")
+    code = _lib._TORCH_TO_CODE
+    return _lib.RouteProblem(T, E, topk, num_expert_group, topk_group, code[dtype],
+                             0 if bias is None else code[bias[1]], code[ids_dtype],
+                             code[weights_dtype], _SCORING[scoring_func],
+                             _GROUP_SCORE[group_score], 1 if renormalize else 0, scale)
+
+
 def grouped_topk(gating_output: torch.Tensor, topk: int, renormalize: bool,
                  num_expert_group: int = 1, topk_group: int = 1, *,
                  scoring_func: str = "softmax", correction_bias: torch.Tensor | None = None,
@@ -205,30 +242,11 @@ def grouped_topk(gating_output: torch.Tensor, topk: int, renormalize: bool,
     (int32, one element on the device) on, the padding of a captured batch.
     Stream-ordered, graph-capturable, no workspace, no backward.
     """
-    if gating_output.dim() != 2:
-        raise ValueError("gating_output must be [T, E]")
-    if gating_output.dtype not in _FLOAT_DTYPES:
-        raise ValueError("gating_output must be float32, float16 or bfloat16")
-    T, E = gating_output.shape
-    if not 1 <= E <= 1024:
-        raise ValueError(f"E={E} experts is not in [1, 1024]")
-    if not 1 <= num_expert_group <= 64 or E % num_expert_group:
-        raise ValueError(f"num_expert_group={num_expert_group} must divide E={E} and be at most 64")
-    if not 1 <= topk_group <= num_expert_group:
-        raise ValueError(f"topk_group={topk_group} must be in [1, num_expert_group]")
-    if not 1 <= topk <= min(64, E // num_expert_group * topk_group):
-        raise ValueError(f"topk={topk} must be in [1, 64] and fit the experts of topk_group groups")
-    if scoring_func not in _SCORING:
-        raise ValueError(f"unsupported scoring_func {scoring_func!r}")
-    if group_score is None:
-        group_score = "max" if correction_bias is None else "top2"
-    if group_score not in _GROUP_SCORE:
-        raise ValueError(f"unsupported group_score {group_score!r}")
-    if ids_dtype not in (torch.int32, torch.int64) or weights_dtype not in _FLOAT_DTYPES:
-        raise ValueError("ids must be int32 or int64, weights float32, float16 or bfloat16")
-    if correction_bias is not None and (correction_bias.dtype not in _FLOAT_DTYPES
-                                        or tuple(correction_bias.shape) != (E,)):
-        raise ValueError(f"correction_bias must be [{E}], float32, float16 or bfloat16")
+    p = _route_problem(
+        gating_output.shape, gating_output.dtype,
+        None if correction_bias is None else (correction_bias.shape, correction_bias.dtype), topk,
+        renormalize, num_expert_group, topk_group, scoring_func, group_score,
+        float(routed_scaling_factor), ids_dtype, weights_dtype)
     if num_token_non_padded is not None and (num_token_non_padded.dtype != torch.int32
                                              or num_token_non_padded.numel() != 1):
         raise ValueError("num_token_non_padded must be one int32 element on the device")
@@ -237,15 +255,10 @@ def grouped_topk(gating_output: torch.Tensor, topk: int, renormalize: bool,
         raise ValueError("grouped_topk has no backward: call it under torch.no_grad()")
     g = gating_output if gating_output.is_contiguous() else gating_output.contiguous()
     dev = _lib.require_gpu(g, correction_bias, num_token_non_padded)
+    T = p.n_tokens
     ids = torch.empty(T, topk, dtype=ids_dtype, device=dev)
     wts = torch.empty(T, topk, dtype=weights_dtype, device=dev)
-    code = _lib._TORCH_TO_CODE
-    p = _lib.route_problem(T, E, topk, num_expert_group, topk_group, code[g.dtype],
-                           0 if correction_bias is None else code[correction_bias.dtype],
-                           code[ids_dtype], code[weights_dtype], _SCORING[scoring_func],
-                           _GROUP_SCORE[group_score], 1 if renormalize else 0,
-                           float(routed_scaling_factor))
     _lib.launch(_lib.lib().exq_grouped_topk,
                 (p, g.data_ptr(), _lib.ptr(correction_bias), _lib.ptr(num_token_non_padded),
-                 ids.data_ptr(), wts.data_ptr()), g.get_device(), "grouped_topk")
+                 ids.data_ptr(), wts.data_ptr()), dev.index, "grouped_topk")
     return wts, ids

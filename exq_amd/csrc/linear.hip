@@ -20,6 +20,7 @@ struct LinArgs {
   int64_t T, N, K;             // N: output columns
   int bdt, rdt, odt, act;
   int vec_b, vec_r, vec_o;     // four consecutive elements may be accessed at once
+  int odd;                     // rows of x or W may start at an odd 2-byte address
 };
 
 template <bool BF>
@@ -600,25 +601,63 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(LinArgs a, in
 }
 
 // ---- any layout --------------------------------------------------------------------
-// Rows that are not 16-byte aligned, or K % 8 != 0: no copies into LDS, but unaligned
-// 16-byte loads.  Eight consecutive elements [k, k + 8) of a row, zeros from K on.
+// Rows that are not 16-byte aligned, or K % 8 != 0: no copies into LDS, but 16-byte
+// loads.  From 4-byte aligned addresses they cost little more than aligned ones, from odd
+// 2-byte addresses twice as much; a row at an odd one (`odd`: there may be such) is read
+// from two bytes before, and its pieces are shifted together (60 tokens x 2049 x 5632 53 ->
+// 23 us).  All bytes read lie within the tensors' storage.  The tiles load odd rows as
+// they lie: shifting took them longer (4096 x 4095 x 4096 249 -> 286 us).
 struct __attribute__((packed, aligned(2))) Chunk {
   uint32_t d[4];
 };
-__device__ __forceinline__ uint4 load_chunk(const uint16_t* row, int k, int K) {
-  if (k + 8 <= K) {
-    const Chunk c = *reinterpret_cast<const Chunk*>(row + k);
-    return uint4{c.d[0], c.d[1], c.d[2], c.d[3]};
-  }
+__device__ __forceinline__ uint4 load_unaligned(const uint16_t* p) {
+  const Chunk c = *reinterpret_cast<const Chunk*>(p);
+  return uint4{c.d[0], c.d[1], c.d[2], c.d[3]};
+}
+struct __attribute__((aligned(4))) Quad {
+  uint32_t d[4];
+};
+__device__ __forceinline__ uint4 load_quad(const uint16_t* p) {
+  const Quad c = *reinterpret_cast<const Quad*>((uintptr_t)p & ~(uintptr_t)3);
+  return uint4{c.d[0], c.d[1], c.d[2], c.d[3]};
+}
+// Bits [sh, sh + 128) of c followed by `next`, sh = 0 or 16.
+__device__ __forceinline__ uint4 shift_quad(const uint4& c, uint32_t next, uint32_t sh) {
+  return uint4{__builtin_amdgcn_alignbit(c.y, c.x, sh), __builtin_amdgcn_alignbit(c.z, c.y, sh),
+               __builtin_amdgcn_alignbit(c.w, c.z, sh), __builtin_amdgcn_alignbit(next, c.w, sh)};
+}
+__device__ __forceinline__ uint32_t odd_shift(const uint16_t* p) {
+  return (uint32_t)((uintptr_t)p & 2) * 8;
+}
+// Eight consecutive elements [k, k + 8) of a row, one by one, zeros from K on.
+__device__ __forceinline__ uint4 load_tail(const uint16_t* row, int k, int K) {
   uint32_t d[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     if (k + j < K) d[j >> 1] |= (uint32_t)row[k + j] << ((j & 1) * 16);
   return uint4{d[0], d[1], d[2], d[3]};
 }
+// U chunks of eight from element k on.
+template <int U>
+__device__ __forceinline__ void load_chunks(const uint16_t* row, int k, int K, bool odd,
+                                            uint4 (&v)[U]) {
+  if (k + 8 * U <= K) {
+    const uint32_t last = odd ? row[k + 8 * U - 1] : 0u;
+#pragma unroll
+    for (int i = 0; i < U; ++i) v[i] = load_quad(row + k + 8 * i);
+    const uint32_t sh = odd ? odd_shift(row + k) : 0u;
+#pragma unroll
+    for (int i = 0; i < U; ++i) v[i] = shift_quad(v[i], i + 1 < U ? v[i + 1].x : last, sh);
+  } else {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      v[i] = k + 8 * i + 8 <= K ? load_unaligned(row + k + 8 * i) : load_tail(row, k + 8 * i, K);
+  }
+}
 
-// Few tokens: as linear_stream_kernel, the matrix operands straight from memory.
-// Wave w takes the 32-k steps w, w + W, ..., U of them in flight.
+// Few tokens: as linear_stream_kernel, the matrix operands straight from memory.  Wave
+// w takes the 32 U-k steps w, w + W, ...; lane quarter q holds 8 U consecutive k of each
+// row, eight of them in each matrix instruction.
 template <bool BF, bool GATED, int MT, int NT, int W, int U>
 __global__ void __launch_bounds__(64 * W) linear_stream_any_kernel(LinArgs a, int nm, int nn) {
   constexpr int TILES = GATED ? NT / 2 : NT;
@@ -634,30 +673,27 @@ __global__ void __launch_bounds__(64 * W) linear_stream_any_kernel(LinArgs a, in
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int64_t m = m0 + t * 16 + r16;
-    xp[t] = a.x + (m < a.T ? m : a.T - 1) * a.ldx + q * 8;
+    xp[t] = a.x + (m < a.T ? m : a.T - 1) * a.ldx;
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int64_t n = n0 + run_col<TILES>(t % TILES, r16);
-    wp[t] = a.w + ((n < a.N ? n : a.N - 1) + (t >= TILES ? a.N : 0)) * a.ldw + q * 8;
+    wp[t] = a.w + ((n < a.N ? n : a.N - 1) + (t >= TILES ? a.N : 0)) * a.ldw;
   }
   f32x4_t acc[MT][NT] = {};
-  for (int k0 = wave * 32; k0 < K; k0 += 32 * W * U) {
-    uint4 x[U][MT], w[U][NT];
+  for (int k0 = wave * 32 * U; k0 < K; k0 += 32 * U * W) {
+    const int k = k0 + q * 8 * U;
+    uint4 x[MT][U], w[NT][U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int k = k0 + i * 32 * W, left = K - q * 8;
+    for (int t = 0; t < NT; ++t) load_chunks<U>(wp[t], k, K, a.odd, w[t]);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) w[i][t] = load_chunk(wp[t], k, left);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) x[i][t] = load_chunk(xp[t], k, left);
-    }
+    for (int t = 0; t < MT; ++t) load_chunks<U>(xp[t], k, K, a.odd, x[t]);
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int u = 0; u < MT; ++u) acc[u][t] = mfma<BF>(w[i][t], x[i][u], acc[u][t]);
+        for (int u = 0; u < MT; ++u) acc[u][t] = mfma<BF>(w[t][i], x[u][i], acc[u][t]);
   }
   join_waves<GATED, MT, NT, W>(a, red, acc, m0, n0, wave, lane);
 }
@@ -698,18 +734,20 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_tile_any_kernel(LinArgs a
   const int xo = (wm * MT * 32 + r32) * 128, wo = BM * 128 + (wn * NT * 32 + r32) * 128;
   const int sw = swz(r32) * 16, hb = h * 16;
   uint4 v[D];
+  auto load = [&](int b) {
+    const int k = b * KB + ch * 8;
 #pragma unroll
-  for (int j = 0; j < D; ++j) v[j] = load_chunk(rows[j], ch * 8, K);
+    for (int j = 0; j < D; ++j)
+      v[j] = k + 8 <= K ? load_unaligned(rows[j] + k) : load_tail(rows[j], k, K);
+  };
+  load(0);
   const int nk = (K + KB - 1) / KB;
   for (int kb = 0; kb < nk; ++kb) {
     unsigned char* stage = lds + (kb & 1) * STAGE;
 #pragma unroll
     for (int j = 0; j < D; ++j) *reinterpret_cast<uint4*>(stage + at[j]) = v[j];
     __syncthreads();  // (the stage written next was read before this)
-    if (kb + 1 < nk) {
-#pragma unroll
-      for (int j = 0; j < D; ++j) v[j] = load_chunk(rows[j], (kb + 1) * KB + ch * 8, K);
-    }
+    if (kb + 1 < nk) load(kb + 1);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const unsigned char* p = stage + ((s * 32 + hb) ^ sw);
@@ -882,6 +920,7 @@ extern "C" int exq_linear(const exq_linear_problem* p, const void* x, const void
   a.vec_b = (uintptr_t)bias % 16 == 0 && up % 4 == 0;
   a.vec_r = (uintptr_t)residual % 16 == 0 && p->residual_stride % 4 == 0;
   a.vec_o = (uintptr_t)out % 16 == 0 && p->out_stride % 4 == 0;
+  a.odd = ((uintptr_t)x | (uintptr_t)weight) % 4 != 0 || (a.ldx | a.ldw) % 2 != 0;
   const hipStream_t s = as_stream(stream);
   if (p->act_dtype == EXQ_DTYPE_BF16)
     return p->gated ? launch_linear<true, true>(a, s) : launch_linear<true, false>(a, s);

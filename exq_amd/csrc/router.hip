@@ -626,7 +626,7 @@ extern "C" int exq_grouped_topk(const exq_route_problem* p, const void* logits, 
               "%s: scoring=%d is neither softmax nor sigmoid", fn, p->scoring);
   EXQ_REQUIRE(p->group_score == EXQ_GROUP_MAX || p->group_score == EXQ_GROUP_TOP2,
               "%s: group_score=%d is neither max nor top2", fn, p->group_score);
-  EXQ_REQUIRE(p->n_tokens >= 0 && p->n_tokens <= INT32_MAX / 4, "%s: n_tokens=%lld out of range",
+  EXQ_REQUIRE(p->n_tokens >= 0 && p->n_tokens < (1 << 26), "%s: n_tokens=%lld out of range",
               fn, (long long)p->n_tokens);
   EXQ_REQUIRE(p->n_experts >= 1 && p->n_experts <= 1024, "%s: n_experts=%lld must be in [1, 1024]",
               fn, (long long)p->n_experts);

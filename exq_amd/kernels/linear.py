@@ -115,7 +115,8 @@ def _call(x, weight, bias, activation, residual, out_dtype, out, gated, what):
                  _layout(bias), _layout(residual), _layout(out), out_dtype, activation, gated)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+                                    or (residual is not None and residual.requires_grad)
+                                    or (out is not None and out.requires_grad)):
         raise ValueError(f"{what} has no backward: call it under torch.no_grad()")
     dev = x.get_device()
     if dev < 0:

@@ -98,7 +98,7 @@ int exq_topk_softmax(const void* logits, int logits_dtype, int64_t n_tokens,
  * largest finite float.  Slots for which no expert is left get id -1 (dropped by
  * the layers) and weight 0, and so do all slots of the rows from *n_valid on
  * (nullable, a device value: the padding of a captured batch).
- * n_experts <= 1024, n_groups <= 64, top_k <= 64.  No workspace.
+ * n_tokens < 2^26, n_experts <= 1024, n_groups <= 64, top_k <= 64.  No workspace.
  */
 typedef enum exq_scoring { EXQ_SCORE_SOFTMAX = 0, EXQ_SCORE_SIGMOID = 1 } exq_scoring;
 typedef enum exq_group_score { EXQ_GROUP_MAX = 0, EXQ_GROUP_TOP2 = 1 } exq_group_score;

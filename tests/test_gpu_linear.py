@@ -232,6 +232,59 @@ def test_large_offsets(device):
     _exact(x2, w, None, None, out, False)
 
 
+def test_two_streams_at_once(device):
+    """Calls on two streams, each kernel shape, and calls from tensors made on another
+    stream: nothing is shared between them."""
+    from exq_amd.kernels import fused_gated_linear, fused_linear
+    banner("linear two streams")
+    sizes = [(1, 2048, 512), (40, 1024, 256), (100, 777, 300), (300, 512, 640), (1100, 256, 2048),
+             (2300, 320, 4100)]
+    data = []
+    for T, K, N in sizes:
+        x, w = _ints((T, K), 1, torch.bfloat16).cuda(), _ints((2 * N, K), 2, torch.bfloat16, 1).cuda()
+        data.append((x, w, fused_linear(x, w, out_dtype=torch.float32),
+                     fused_gated_linear(x, w, activation="relu")))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                for x, w, a, b in (data if i == 0 else data[::-1]):
+                    outs.append((fused_linear(x, w, out_dtype=torch.float32), a))
+                    outs.append((fused_gated_linear(x, w, activation="relu"), b))
+    torch.cuda.synchronize()
+    for got, want in outs:
+        assert torch.equal(got, want)
+
+
+def test_every_width_near_the_tiles(device):
+    """T and N one below, at and above each tile's edges, K around a step."""
+    from exq_amd.kernels import fused_linear
+    banner("linear edges")
+    for T in (255, 256, 257, 383, 385):
+        for N in (255, 256, 257, 513):
+            for K in (56, 64, 72, 120, 136):
+                x, w = _ints((T, K), T, torch.bfloat16).cuda(), _ints((N, K), N, torch.bfloat16).cuda()
+                _exact(x, w, None, None, fused_linear(x, w, out_dtype=torch.float32), False)
+
+
+@pytest.mark.parametrize("T,K,N", [(2500, 192, 4096), (4100, 136, 4352), (1030, 4096, 520),
+                                   (20000, 64, 128), (3, 16384, 72)])
+def test_large_shapes_whole_numbers(T, K, N, device):
+    """The largest tiles with ragged edges, long contractions, many token blocks."""
+    from exq_amd.kernels import fused_gated_linear, fused_linear
+    banner(f"large shapes T={T} K={K} N={N}")
+    x, w = _ints((T, K), 1, torch.bfloat16, 1).cuda(), _ints((N, K), 2, torch.bfloat16, 1).cuda()
+    r = _ints((T, N), 3, torch.bfloat16, 90).cuda()
+    out = fused_linear(x, w, residual=r, out_dtype=torch.float32)
+    y = x.double() @ w.double().t()
+    assert torch.equal(out, (y + r.double()).float())
+    half = N // 2 * 2
+    g = fused_gated_linear(x, w[:half], activation="relu", out_dtype=torch.float32)
+    assert torch.equal(g, (torch.relu(y[:, :half // 2]) * y[:, half // 2:half]).float())
+
+
 def test_moe_block(device):
     """The operators together, as a block runs them: router projection, grouped routing,
     routed experts, shared expert with its output added onto theirs; eager, and captured

@@ -109,6 +109,7 @@ def test_linear_refusals():
                      ((x, w), dict(activation="tanh")),
                      ((x, w), dict(residual=torch.zeros(4, 7))),
                      ((x, w), dict(residual=torch.zeros(4, 8, dtype=torch.float64))),
+                     ((x, w), dict(out=torch.zeros(4, 8, dtype=torch.bfloat16).requires_grad_())),
                      ((x, w.clone().requires_grad_()), {})]:
         with pytest.raises(ValueError):
             fused_linear(*args, **kw)
@@ -152,7 +153,8 @@ def test_c_entries_check_arguments():
                      (dict(scoring=2), b"scoring"), (dict(group_score=-1), b"group_score"),
                      (dict(n_experts=1025), b"n_experts"), (dict(n_groups=3), b"n_groups"),
                      (dict(topk_group=5), b"topk_group"), (dict(top_k=9), b"top_k"),
-                     (dict(n_tokens=-1), b"n_tokens"), ({}, b"null pointer")]:
+                     (dict(n_tokens=-1), b"n_tokens"), (dict(n_tokens=1 << 26), b"n_tokens"),
+                     ({}, b"null pointer")]:
         st, msg = route(**kw)
         assert st == 1 and text in msg, (kw, msg)
 

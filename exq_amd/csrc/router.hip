@@ -274,7 +274,7 @@ __device__ __forceinline__ float min_op(float a, float b) { return fminf(a, b); 
 __device__ __forceinline__ float sum_op(float a, float b) { return a + b; }
 // f(constant I), ... f(constant N - 1)
 template <int I, int N, typename F>
-__device__ __forceinline__ void unrolled(F f) {
+__device__ __forceinline__ void unrolled(F&& f) {
   if constexpr (I < N) {
     f(std::integral_constant<int, I>{});
     unrolled<I + 1, N>(f);
@@ -301,11 +301,11 @@ __device__ __forceinline__ float4 load4(const void* p, int dt, int64_t i) {
 }
 
 // The k best of a row's keys, lane l holding those of experts e0 .. e0 + CH - 1 (-inf:
-// none): candidates c[i] with their ranks, slot i * 16 + l of `total`.
+// none): candidates c[i], every key from V on, with their ranks, slot i * 16 + l of `total`.
 template <int CH, int KC>
 __device__ __forceinline__ void rank_experts(const float (&key)[CH], int e0, int k, int lane,
                                              Candidate* cand, Candidate (&c)[KC], int (&rank)[KC],
-                                             int& total) {
+                                             int& total, float& V) {
   const int l16 = lane & 15;
   // V: the largest of the lanes' two best that k + 1 of them reach
   float m1 = -INFINITY, m2 = -INFINITY;
@@ -321,7 +321,7 @@ __device__ __forceinline__ void rank_experts(const float (&key)[CH], int e0, int
     c1 += (o1 >= m1 ? 1 : 0) + (o2 >= m1 ? 1 : 0);
     c2 += (o1 >= m2 ? 1 : 0) + (o2 >= m2 ? 1 : 0);
   });
-  float V = row_reduce<16>(c1 > k ? m1 : c2 > k ? m2 : -INFINITY, max_op);
+  V = row_reduce<16>(c1 > k ? m1 : c2 > k ? m2 : -INFINITY, max_op);
   V = fmaxf(V, -FLT_MAX);  // (an expert that is there has a key above -inf)
   int cnt = 0;
 #pragma unroll
@@ -370,9 +370,15 @@ __device__ __forceinline__ void rank_experts(const float (&key)[CH], int e0, int
 // and |x| e^-|x| <= 0.37, x s (1 - s) <= 0.23, so a sigmoid s is off by at most 4 and e / S
 // by 3 / S + 58 s (S: a weighted mean of |x| is at most ln 512, 36 additions); adding the
 // bias rounds once.  A ranking between two values no further apart than both bounds
-// together is left to route_row (`tol`: 9 and 128 / S for the scores, a little over 2 |r|
-// for the rounded sums); a sum of two scores has twice that.  With logits as they come
-// and a small bias that is about one row in 3,000.
+// together is made in 64 bits (`tol`: 9 and 128 / S for the scores, a little over 2 |r|
+// for the rounded sums): among the candidates where it is theirs (sigmoid), by route_row
+// otherwise.  A sum of two scores has twice the bound.  With logits as they come and a
+// small bias that is one row in some thousands, but then most batches have one, and the
+// wave that does is the last to end: 4,096 tokens 12.7 us with route_row alone.
+// The largest instance has room for one of the two widths of the second deal.
+template <int CH, int G, int KC>
+constexpr bool kHalfOnly = CH == 32 && G == 16 && KC == 2;
+
 template <int CH, int G, int KC, int MAXC>
 __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
   constexpr int LG = 16 / G;       // lanes of a group
@@ -438,7 +444,7 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
     S = row_reduce<16>(S, sum_op);
   }
   const float rS = __builtin_amdgcn_rcpf(S);
-  auto score = [&](float x) {  // (0 for -inf)
+  auto score = [&](float x) __attribute__((always_inline)) {  // (0 for -inf)
     return a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-x * kLog2e))
                      : __builtin_amdgcn_exp2f((x - m) * kLog2e) * rS;
   };
@@ -460,6 +466,7 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
   bool unsure = false;
   Candidate c[KC];
   int rank[KC], total;
+  float V;
 
   if constexpr (G > 1) {
     float v1 = -INFINITY, v2 = -INFINITY;
@@ -498,9 +505,17 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
     }
     // the kept groups, again over all lanes: lanes2 lanes for each of them
     float* keys = s_key[tok];
+    if (CH <= 16 && a.vec) {
 #pragma unroll
-    for (int p = 0; p < CH; ++p)
-      if (p < n) keys[e0 + p] = key[p];
+      for (int p = 0; p < CH; p += 4)
+        if (p < n)
+          *reinterpret_cast<float4*>(keys + e0 + p) =
+              float4{key[p], key[p + 1], key[p + 2], key[p + 3]};
+    } else {
+#pragma unroll
+      for (int p = 0; p < CH; ++p)
+        if (p < n) keys[e0 + p] = key[p];
+    }
     uint32_t kept = (uint32_t)(__ballot(keep && sub == 0) >> (lane & 48)) & 0xffffu;
     const int j = l16 / a.lanes2, sub2 = l16 - j * a.lanes2;
     for (int i = 0; i + 1 < a.top_groups; ++i)
@@ -510,19 +525,33 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
     if (j >= a.top_groups) n2 = 0;
     e0 = g2 * a.gs + first2;
     __builtin_amdgcn_wave_barrier();
-    constexpr int H = CH / 2;
-    if (a.chunk2 <= H) {
+    auto deal = [&](auto& to, auto size) __attribute__((always_inline)) {
+      constexpr int N = decltype(size)::value;
+      if (CH <= 16 && a.vec) {
+#pragma unroll
+        for (int p = 0; p < N; p += 4) {
+          const float4 v = p < n2 ? *reinterpret_cast<const float4*>(keys + e0 + p)
+                                  : float4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          to[p] = v.x; to[p + 1] = v.y; to[p + 2] = v.z; to[p + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < N; ++p) to[p] = p < n2 ? keys[e0 + p] : -INFINITY;
+      }
+      rank_experts<N, KC>(to, e0, a.k, lane, s_cand[tok], c, rank, total, V);
+    };
+    constexpr int H = CH >= 8 ? CH / 2 : CH;
+    if constexpr (kHalfOnly<CH, G, KC>) {
       float half[H];
-#pragma unroll
-      for (int p = 0; p < H; ++p) half[p] = p < n2 ? keys[e0 + p] : -INFINITY;
-      rank_experts<H, KC>(half, e0, a.k, lane, s_cand[tok], c, rank, total);
+      deal(half, std::integral_constant<int, H>{});
+    } else if (CH >= 8 && a.chunk2 <= H) {
+      float half[H];
+      deal(half, std::integral_constant<int, H>{});
     } else {
-#pragma unroll
-      for (int p = 0; p < CH; ++p) key[p] = p < n2 ? keys[e0 + p] : -INFINITY;
-      rank_experts<CH, KC>(key, e0, a.k, lane, s_cand[tok], c, rank, total);
+      deal(key, std::integral_constant<int, CH>{});
     }
   } else {
-    rank_experts<CH, KC>(key, e0, a.k, lane, s_cand[tok], c, rank, total);
+    rank_experts<CH, KC>(key, e0, a.k, lane, s_cand[tok], c, rank, total, V);
   }
   unsure |= total > 16 * KC;
   if (a.bias) {  // keys are rounded scores: is one of the first k next to its follower?
@@ -530,12 +559,50 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
 #pragma unroll
     for (int i = 0; i < KC; ++i) sorted[rank[i]] = c[i].key;
     __builtin_amdgcn_wave_barrier();
+    bool close = false;
 #pragma unroll
-    for (int i = 0; i < KC; ++i)
-      if (rank[i] < a.k && rank[i] + 1 < total) {
-        const float next = sorted[rank[i] + 1];
-        unsure |= !(c[i].key - next > tol0 + 0x1.2p-23f * fabsf(c[i].key));
+    for (int i = 0; i < KC; ++i) {
+      const float tol = tol0 + 0x1.2p-23f * fabsf(c[i].key);
+      if (rank[i] < a.k && rank[i] + 1 < total) close |= !(c[i].key - sorted[rank[i] + 1] > tol);
+      // next to what is no candidate: then the row is not these candidates' to decide
+      if (rank[i] == a.k - 1 && i * 16 + l16 < total) unsure |= !(c[i].key - V > tol);
+    }
+    constexpr bool kAgain = CH <= 16 || KC == 1;  // (registers)
+    if (!kAgain || !a.sigmoid) {
+      unsure |= close;
+    } else if (__ballot(close)) {  // the candidates again, ranked by their scores in 64 bits
+      double r[KC];
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        r[i] = -INFINITY;
+        if (i * 16 + l16 < total) {
+          const float x = fminf(load_as_f32(a.logits, a.ldt, rr * a.E + c[i].id), FLT_MAX);
+          r[i] = 1.0 / (1.0 + exp(-(double)x)) + (double)load_as_f32(a.bias, a.bdt, c[i].id);
+        }
+        rank[i] = 0;
       }
+      auto first_of = [](double o, int oid, double x, int id) {
+        return o > x || (o == x && oid < id) ? 1 : 0;
+      };
+#pragma unroll
+      for (int i = 0; i < KC; ++i)
+#pragma unroll
+        for (int j = 0; j < KC; ++j)
+          if (i != j) rank[i] += first_of(r[j], c[j].id, r[i], c[i].id);
+      unrolled<1, 16>([&](auto n) {
+        constexpr int CTRL = 0x120 + decltype(n)::value;
+#pragma unroll
+        for (int j = 0; j < KC; ++j) {
+          const uint64_t u = (uint64_t)__double_as_longlong(r[j]);
+          const double o = __longlong_as_double(
+              (long long)((uint64_t)(uint32_t)rowi<CTRL>((int)(u >> 32)) << 32 |
+                          (uint32_t)rowi<CTRL>((int)(uint32_t)u)));
+          const int oid = rowi<CTRL>(c[j].id);
+#pragma unroll
+          for (int i = 0; i < KC; ++i) rank[i] += first_of(o, oid, r[i], c[i].id);
+        }
+      });
+    }
   }
 
   // weights of the chosen: rank < k and an expert in the slot
@@ -584,9 +651,19 @@ int launch_tokens(const RouteArgs& a, hipStream_t s) {
                      dim3((unsigned)cdiv(a.T, 16)), dim3(256), 0, s, a);
   return check_launch("route_tokens_kernel");
 }
+int launch_rows(const RouteArgs& a, hipStream_t s) {
+  const dim3 g((unsigned)cdiv(a.T, 4));
+  if (a.E <= 256)
+    hipLaunchKernelGGL(route_rows_kernel<4>, g, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(route_rows_kernel<16>, g, dim3(256), 0, s, a);
+  return check_launch("route_rows_kernel");
+}
 template <int CH, int G>
 int launch_slots(const RouteArgs& a, hipStream_t s) {
-  return a.k <= 10 ? launch_tokens<CH, G, 1>(a, s) : launch_tokens<CH, G, 2>(a, s);
+  if (a.k <= 10) return launch_tokens<CH, G, 1>(a, s);
+  if (kHalfOnly<CH, G, 2> && a.chunk2 > CH / 2) return launch_rows(a, s);
+  return launch_tokens<CH, G, 2>(a, s);
 }
 template <int G>
 int launch_chunk(RouteArgs a, hipStream_t s) {
@@ -599,6 +676,7 @@ int launch_chunk(RouteArgs a, hipStream_t s) {
       (uintptr_t)a.logits % (4 * dtype_bytes(a.ldt)) == 0 &&
       (!a.bias || (uintptr_t)a.bias % (4 * dtype_bytes(a.bdt)) == 0)) {
     a.chunk = up;
+    a.chunk2 = (a.chunk2 + 3) / 4 * 4;  // (no more than chunk: a kept group has as many lanes)
     a.vec = 1;
   }
   if (a.chunk <= 4) return launch_slots<4, G>(a, s);
@@ -678,10 +756,5 @@ extern "C" int exq_grouped_topk(const exq_route_problem* p, const void* logits, 
       if (G == 16) return launch_chunk<16>(f, s);
     }
   }
-  const dim3 g((unsigned)cdiv(a.T, 4));
-  if (a.E <= 256)
-    hipLaunchKernelGGL(route_rows_kernel<4>, g, dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL(route_rows_kernel<16>, g, dim3(256), 0, s, a);
-  return check_launch("route_rows_kernel");
+  return launch_rows(a, s);
 }

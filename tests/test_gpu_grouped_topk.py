@@ -75,6 +75,8 @@ SHAPES = [  # T, E, k, groups, kept
     (17, 60, 4, 1, 1), (9, 72, 8, 4, 2), (50, 512, 16, 16, 5), (7, 1024, 64, 32, 9),
     (40, 96, 5, 3, 2), (21, 20, 3, 10, 4), (4, 16, 2, 16, 2), (3, 8, 8, 8, 8), (2, 2, 1, 2, 1),
     (6, 1, 1, 1, 1), (130, 288, 16, 8, 3), (66, 352, 12, 16, 11), (12, 640, 10, 64, 7),
+    (20, 512, 12, 16, 11), (9, 512, 24, 16, 4), (11, 256, 24, 8, 3), (9, 512, 30, 8, 4), (300, 256, 10, 8, 1),
+    (33, 512, 11, 16, 8), (5, 384, 25, 4, 2), (40, 112, 9, 16, 5),
 ]
 
 
@@ -126,6 +128,28 @@ def test_near_ties_are_decided_in_64_bits(device):
         _check(lg, 8, True, 8, 4, scoring, bias)
         _check(lg, 8, False, 8, 4, scoring, None, "top2")
         _check(lg, 6, False, 1, 1, scoring, bias)
+
+
+@pytest.mark.parametrize("k", [1, 6, 10, 11, 24])
+def test_few_near_ties(k, device):
+    """Two scores or two groups of some rows a rounding apart, the others far: among the
+    chosen, at the k-th place, below it, and where one is no candidate."""
+    banner(f"grouped_topk few near ties k={k}")
+    rng = np.random.default_rng(k)
+    for E, G, keep in ((256, 1, 1), (256, 8, 4), (96, 4, 2), (512, 16, 12)):
+        T = 200
+        lg = rng.standard_normal((T, E)).astype(np.float32)
+        bias = (0.05 * rng.standard_normal(E)).astype(np.float32)
+        r = 1 / (1 + np.exp(-lg.astype(np.float64))) + bias
+        order = np.argsort(-r, axis=1)
+        for t in range(T):   # expert b's logit set so that its rank value is a's, or next to it
+            i = rng.integers(0, min(E - 2, k + 3))
+            a, b = order[t, i], order[t, i + 1 + int(rng.integers(0, 2))]
+            s = min(max(r[t, a] - bias[b], 1e-3), 1 - 1e-3) + rng.integers(-2, 3) * 2.0 ** -26
+            lg[t, b] = np.float32(np.log(s / (1 - s)))
+        _check(torch.from_numpy(lg), k, True, G, keep, "sigmoid", torch.from_numpy(bias))
+        _check(torch.from_numpy(lg), k, False, G, keep, "sigmoid", torch.from_numpy(bias), "max")
+        _check(torch.from_numpy(lg), k, True, G, keep, "softmax", torch.from_numpy(bias / E))
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])

@@ -570,9 +570,11 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(LinArgs a, in
       }
     }
   } else {
-    // the copies of a block: over the step that follows the meeting and the next CS - 1
-    // (with two stages one step less, which is what their last copies have to land)
-    constexpr int CS = NST == 2 && STEPS > 2 ? STEPS - 1 : STEPS;
+    // The copies of a block: over the step that follows the meeting and the next CS - 1.
+    // With two stages the last ones need the rest of the block to land; four waves, with
+    // twice the copies each, stall on issue when they are closer together (192 x 256, 8
+    // waves: two steps 55.1 us, three 56.3; 256 x 256, 4 waves: 95.8 and 90.0).
+    constexpr int CS = NST > 2 ? STEPS : W == 8 ? 2 : 3;
 #pragma unroll
     for (int i = 0; i < R; ++i) read(0, 0, 0, i);
     int prev = (NST - 1) * STAGE;  // (before the first meeting: its last blocks once more)
@@ -859,7 +861,7 @@ int launch_linear(const LinArgs& a, hipStream_t s) {
       case 4: return launch_tile<BF, GATED, 2, 2, 1, 2, 6, 0, true>(a, s);
       case 5: return launch_tile<BF, GATED, 2, 4, 2, 1, 4, 0, true>(a, s);
       case 6: return launch_tile<BF, GATED, 2, 4, 2, 2, 3, 0, false>(a, s);
-      case 7: return launch_tile<BF, GATED, 2, 4, 3, 2, 2, 0, false>(a, s);
+      case 7: return launch_tile<BF, GATED, 2, 4, 3, 2, 2, 3, false>(a, s);
       default: return launch_tile<BF, GATED, 2, 2, 4, 4, 2, 4, false>(a, s);
     }
   }

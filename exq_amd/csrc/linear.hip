@@ -816,7 +816,9 @@ int launch_tile_any(const LinArgs& a, hipStream_t s) {
 // CUs hold one, `ns2` when they hold two (0: they cannot), measured in bf16 with K = 2048
 // (256 x 256: 4096 and 14336); it does not move with K.  The stream kernels win while
 // their rounds are few (64 tokens x 2816 gated columns: 64-token streams 11.8 us, 64 x 64
-// tiles 14.0; 100 tokens: 17.5 and 13.0), small tiles until they need a further round
+// tiles 14.0; 100 tokens: 17.5 and 13.0), those of 16 rows while they fit one round (16
+// tokens x 4096 x 4096: 16 rows 9.6 us, 32 rows 13.6; x 8192 x 8192: 31.7 and 30.4; 64
+// tokens x 2816 x 2048: 32 x 16 8.5, 32 x 32 9.8, 64 x 32 12.7), small tiles until they need a further round
 // (1024 tokens x 2048 x 2048: 64 x 128 18.4 us, 128 x 128 21.5, 256 x 256 59; 2001 tokens x
 // 2048 x 5632: 192 x 256 56.5 us, 256 x 256 60, 128 x 256 and 128 x 128 66; 2048 x 4096 x
 // 4096: 128 x 256 64 us, 128 x 128 78, 256 x 256 92).
@@ -827,14 +829,16 @@ constexpr Shape kShapes[] = {
     {16, 32, 140, 0},   {32, 32, 175, 0},    {64, 32, 240, 0},     // streams
     {64, 64, 340, 540}, {64, 128, 470, 0},   {128, 128, 590, 0},   // tiles
     {128, 256, 950, 0}, {192, 256, 1500, 0}, {256, 256, 1740, 0},
+    {16, 16, 100, 0},   {32, 16, 135, 0},    // streams of one weight tile, not for gated rows
 };
 constexpr int kCus = 256;
 
-int pick_shape(int64_t tokens, int64_t rows) {
+int pick_shape(int64_t tokens, int64_t rows, bool gated) {
   int best = 0;
   int64_t least = INT64_MAX;
   for (int i = 0; i < (int)(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {
     const Shape& k = kShapes[i];
+    if (gated && k.rows == 16) continue;
     const int64_t units = cdiv(tokens, k.tokens) * cdiv(rows, k.rows);
     const int64_t round = k.ns2 ? 2 * kCus : kCus, rest = units % round;
     const int64_t ns = units / round * (k.ns2 ? k.ns2 : k.ns) +
@@ -853,7 +857,8 @@ int launch_linear(const LinArgs& a, hipStream_t s) {
                        a.ldw % 8 == 0 && a.K % 8 == 0 && span_fits(256, a.ldx, a.K) &&
                        span_fits(256, a.ldw, a.K);
   if (aligned) {
-    switch (pick_shape(a.T, a.N * (GATED ? 2 : 1))) {
+    const int shape = pick_shape(a.T, a.N * (GATED ? 2 : 1), GATED);
+    switch (shape) {
       case 0: return launch_stream<BF, GATED, 1, 2, 8, 3>(a, s);
       case 1: return launch_stream<BF, GATED, 2, 2, 8, 2>(a, s);
       case 2: return launch_stream<BF, GATED, 4, 2, 4, 3>(a, s);
@@ -862,10 +867,18 @@ int launch_linear(const LinArgs& a, hipStream_t s) {
       case 5: return launch_tile<BF, GATED, 2, 4, 2, 1, 4, 0, true>(a, s);
       case 6: return launch_tile<BF, GATED, 2, 4, 2, 2, 3, 0, false>(a, s);
       case 7: return launch_tile<BF, GATED, 2, 4, 3, 2, 2, 3, false>(a, s);
-      default: return launch_tile<BF, GATED, 2, 2, 4, 4, 2, 4, false>(a, s);
+      case 8: return launch_tile<BF, GATED, 2, 2, 4, 4, 2, 4, false>(a, s);
+      default:
+        if constexpr (!GATED) {
+          return shape == 9 ? launch_stream<BF, GATED, 1, 1, 16, 2>(a, s)
+                            : launch_stream<BF, GATED, 2, 1, 8, 3>(a, s);
+        }
     }
   }
   const int64_t rows = a.N * (GATED ? 2 : 1);
+  if constexpr (!GATED) {
+    if (a.T <= 16 && a.N <= 16 * kCus) return launch_stream_any<BF, GATED, 1, 1, 16, 4>(a, s);
+  }
   if (a.T <= 16) return launch_stream_any<BF, GATED, 1, 2, 8, 4>(a, s);
   if (cdiv(a.T, 32) * cdiv(rows, 32) <= 2 * kCus)
     return launch_stream_any<BF, GATED, 2, 2, 8, 2>(a, s);

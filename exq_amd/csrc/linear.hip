@@ -818,10 +818,10 @@ int launch_tile_any(const LinArgs& a, hipStream_t s) {
 // their rounds are few (64 tokens x 2816 gated columns: 64-token streams 11.8 us, 64 x 64
 // tiles 14.0; 100 tokens: 17.5 and 13.0), those of 16 rows while they fit one round (16
 // tokens x 4096 x 4096: 16 rows 9.6 us, 32 rows 13.6; x 8192 x 8192: 31.7 and 30.4; 64
-// tokens x 2816 x 2048: 32 x 16 8.5, 32 x 32 9.8, 64 x 32 12.7), small tiles until they need a further round
-// (1024 tokens x 2048 x 2048: 64 x 128 18.4 us, 128 x 128 21.5, 256 x 256 59; 2001 tokens x
-// 2048 x 5632: 192 x 256 56.5 us, 256 x 256 60, 128 x 256 and 128 x 128 66; 2048 x 4096 x
-// 4096: 128 x 256 64 us, 128 x 128 78, 256 x 256 92).
+// tokens x 2816 x 2048: 32 x 16 8.5, 32 x 32 9.8, 64 x 32 12.7), small tiles until they
+// need a further round (1024 tokens x 2048 x 2048: 64 x 128 18.4 us, 128 x 128 21.5, 256 x
+// 256 59; 2001 tokens x 2048 x 5632: 192 x 256 56.5 us, 256 x 256 60, 128 x 256 and 128 x
+// 128 66; 2048 x 4096 x 4096: 128 x 256 64 us, 128 x 128 78, 256 x 256 92).
 struct Shape {
   int tokens, rows, ns, ns2;
 };
@@ -876,6 +876,8 @@ int launch_linear(const LinArgs& a, hipStream_t s) {
     }
   }
   const int64_t rows = a.N * (GATED ? 2 : 1);
+  // (16 rows a work-group while they fit one round: 7 tokens x 8801 x 1664 22.0 us, 32 rows
+  // 29.6)
   if constexpr (!GATED) {
     if (a.T <= 16 && a.N <= 16 * kCus) return launch_stream_any<BF, GATED, 1, 1, 16, 4>(a, s);
   }

@@ -285,6 +285,25 @@ def test_large_shapes_whole_numbers(T, K, N, device):
     assert torch.equal(g, (torch.relu(y[:, :half // 2]) * y[:, half // 2:half]).float())
 
 
+@pytest.mark.parametrize("T,K,N", [(1, 1032, 4096), (5, 264, 8200), (16, 1096, 4104), (13, 135, 4097),
+                                   (30, 72, 5000), (32, 2112, 2048), (27, 1025, 8200),
+                                   (64, 1160, 1500), (500, 200, 64)])
+def test_few_tokens_wide_whole_numbers(T, K, N, device):
+    """Streams of 16 and of 32 weight rows on both sides of one round, waves without a
+    step of their own, rows of any alignment."""
+    from exq_amd.kernels import fused_gated_linear, fused_linear
+    banner(f"few tokens, wide T={T} K={K} N={N}")
+    for dtype in (torch.bfloat16, torch.float16):
+        x, w = _ints((T, K), 1, dtype, 1).cuda(), _ints((N, K), 2, dtype, 1).cuda()
+        r = _ints((T, N), 3, dtype, 90).cuda()
+        y = x.double() @ w.double().t()
+        out = fused_linear(x, w, residual=r, out_dtype=torch.float32)
+        assert torch.equal(out, (y + r.double()).float())
+        half = N // 2
+        g = fused_gated_linear(x, w[:2 * half], activation="relu", out_dtype=torch.float32)
+        assert torch.equal(g, (torch.relu(y[:, :half]) * y[:, half:2 * half]).float())
+
+
 def test_moe_block(device):
     """The operators together, as a block runs them: router projection, grouped routing,
     routed experts, shared expert with its output added onto theirs; eager, and captured

@@ -300,6 +300,26 @@ __device__ __forceinline__ float4 load4(const void* p, int dt, int64_t i) {
                 f16_bits_to_f32(u.y & 0xffffu), f16_bits_to_f32(u.y >> 16)};
 }
 
+// n >= 1 consecutive values, all loads on their way before the first is used (the last one
+// again from n on): with the type decided at each they waited for one another.
+template <int CH>
+__device__ __forceinline__ void load_each(const void* p, int dt, int64_t i, int n,
+                                          float (&v)[CH]) {
+  if (dt == EXQ_DTYPE_F32) {
+    const float* f = reinterpret_cast<const float*>(p) + i;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) v[c] = f[c < n ? c : n - 1];
+    return;
+  }
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + i;
+  uint32_t u[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) u[c] = h[c < n ? c : n - 1];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+    v[c] = dt == EXQ_DTYPE_BF16 ? __uint_as_float(u[c] << 16) : f16_bits_to_f32(u[c]);
+}
+
 // The k best of a row's keys, lane l holding those of experts e0 .. e0 + CH - 1 (-inf:
 // none): candidates c[i], every key from V on, with their ranks, slot i * 16 + l of `total`.
 template <int CH, int KC>
@@ -415,12 +435,10 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
         }
       }
   } else {
-#pragma unroll
-    for (int p = 0; p < CH; ++p)
-      if (p < n) {
-        l[p] = load_as_f32(a.logits, a.ldt, rr * a.E + e0 + p);
-        if (a.bias) b[p] = load_as_f32(a.bias, a.bdt, e0 + p);
-      }
+    if (n > 0) {
+      load_each<CH>(a.logits, a.ldt, rr * a.E + e0, n, l);
+      if (a.bias) load_each<CH>(a.bias, a.bdt, e0, n, b);
+    }
   }
 #pragma unroll
   for (int p = 0; p < CH; ++p) {

@@ -91,7 +91,16 @@ __device__ __forceinline__ void store_choice(const RouteArgs& a, int64_t row, in
 __device__ __forceinline__ float choice_weight(const RouteArgs& a, float x, float U, float m,
                                                float S) {
   const float d = a.renorm ? U : a.sigmoid ? 0.f : m;
-  const float e = expf(a.sigmoid && x > 0.f ? -x : x - d);
+  float e;
+  if (a.sigmoid && x > 0.f) {
+    e = expf(-x);
+  } else {
+    // (with the rounding of the difference, which is up to 2^-18 of a score of 1e-37)
+    const double wide = (double)x - (double)d;
+    const float near = (float)wide;
+    e = expf(near);
+    if (near > -120.f) e = fmaf(e, (float)(wide - (double)near), e);
+  }
   if (!a.sigmoid) return a.renorm ? e : e / S;
   return x > 0.f ? 1.f / (1.f + e) : e / (1.f + expf(x));
 }
@@ -387,17 +396,23 @@ __device__ __forceinline__ void rank_experts(const float (&key)[CH], int e0, int
 }
 
 // Roundings.  In units of 2^-24: e^x as exp2(x log2 e) is off by 2.5 |x| + 2 of itself,
-// and |x| e^-|x| <= 0.37, x s (1 - s) <= 0.23, so a sigmoid s is off by at most 4 and e / S
-// by 3 / S + 58 s (S: a weighted mean of |x| is at most ln 512, 36 additions); adding the
-// bias rounds once.  A ranking between two values no further apart than both bounds
-// together is made in 64 bits (`tol`: 9 and 128 / S for the scores, a little over 2 |r|
-// for the rounded sums): among the candidates where it is theirs (sigmoid), by route_row
-// otherwise.  A sum of two scores has twice the bound.  With logits as they come and a
-// small bias that is one row in some thousands, but then most batches have one, and the
-// wave that does is the last to end: 4,096 tokens 12.7 us with route_row alone.
-// The largest instance has room for one of the two widths of the second deal.
+// and |x| e^-|x| <= 0.37, x s (1 - s) <= 0.23, so a sigmoid s is off by at most 4, and e / S
+// by 4 / S beside what S is off by: 58 of itself (a weighted mean of |x| is at most ln 512, 36
+// additions), which moves the difference of two scores by 58 of that difference, and that
+// is no more than their biases differ by where the rounding could turn their order round.
+// Adding the bias rounds once.  A ranking between two values no further apart than this
+// is made in 64 bits (`tol`: 9 for sigmoid scores, 10 / S + 64 times the span of the biases
+// for softmax, a little over 2 |r| for the rounded sums): among the candidates where it
+// is theirs, by route_row otherwise.  A sum of two scores has twice the bound.  With
+// logits as they come and a small bias that is one row in some thousands, but then most
+// batches have one, and the wave that does is the last to end: 4,096 tokens 12.7 us with
+// route_row alone.
+// The largest instances have room for one of the two widths of the second deal (two groups
+// always fit half of it).
 template <int CH, int G, int KC>
-constexpr bool kHalfOnly = CH == 32 && G == 16 && KC == 2;
+constexpr bool kHalfOnly = CH == 32 && (G == 2 || G == 16) && KC == 2;
+template <int CH, int G, int KC>
+constexpr bool kFullOnly = CH == 32 && (G == 4 || G == 8) && KC == 2;
 
 template <int CH, int G, int KC, int MAXC>
 __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
@@ -466,7 +481,17 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
     return a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-x * kLog2e))
                      : __builtin_amdgcn_exp2f((x - m) * kLog2e) * rS;
   };
-  const float tol0 = a.sigmoid ? 0x1.2p-21f : 0x1p-17f * rS;
+  float tol0 = a.sigmoid ? 0x1.2p-21f : 0x1.4p-21f * rS;
+  if (a.bias && !a.sigmoid) {
+    float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < CH; ++p) {
+      lo = fminf(lo, l[p] > -INFINITY ? b[p] : INFINITY);
+      hi = fmaxf(hi, l[p] > -INFINITY ? b[p] : -INFINITY);
+    }
+    const float span = row_reduce<16>(hi, max_op) - row_reduce<16>(lo, min_op);
+    tol0 += 0x1p-18f * fmaxf(fminf(span, rS), 0.f);
+  }
   if (a.bias) {
     if (a.sigmoid) {
 #pragma unroll
@@ -562,7 +587,7 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
     if constexpr (kHalfOnly<CH, G, KC>) {
       float half[H];
       deal(half, std::integral_constant<int, H>{});
-    } else if (CH >= 8 && a.chunk2 <= H) {
+    } else if (!kFullOnly<CH, G, KC> && CH >= 8 && a.chunk2 <= H) {
       float half[H];
       deal(half, std::integral_constant<int, H>{});
     } else {
@@ -585,17 +610,19 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
       // next to what is no candidate: then the row is not these candidates' to decide
       if (rank[i] == a.k - 1 && i * 16 + l16 < total) unsure |= !(c[i].key - V > tol);
     }
-    constexpr bool kAgain = CH <= 16 || KC == 1;  // (registers)
-    if (!kAgain || !a.sigmoid) {
-      unsure |= close;
-    } else if (__ballot(close)) {  // the candidates again, ranked by their scores in 64 bits
+    if (const uint64_t some = __ballot(close)) {
+      // the candidates again, ranked by their scores in 64 bits
       double r[KC];
+      float x[KC];
 #pragma unroll
       for (int i = 0; i < KC; ++i) {
         r[i] = -INFINITY;
+        x[i] = 0.f;
         if (i * 16 + l16 < total) {
-          const float x = fminf(load_as_f32(a.logits, a.ldt, rr * a.E + c[i].id), FLT_MAX);
-          r[i] = 1.0 / (1.0 + exp(-(double)x)) + (double)load_as_f32(a.bias, a.bdt, c[i].id);
+          x[i] = fminf(load_as_f32(a.logits, a.ldt, rr * a.E + c[i].id), FLT_MAX);
+          const double e = exp(a.sigmoid ? -(double)x[i] : (double)x[i] - (double)m);
+          r[i] = (a.sigmoid ? 1.0 / (1.0 + e) : e / (double)S) +
+                 (double)load_as_f32(a.bias, a.bdt, c[i].id);
         }
         rank[i] = 0;
       }
@@ -620,6 +647,27 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
           for (int i = 0; i < KC; ++i) rank[i] += first_of(o, oid, r[i], c[i].id);
         }
       });
+      if (!a.sigmoid) {
+        // S has the rounding of 32 bits, 2^-18 of it, which moves the difference of two
+        // values by that much of the difference of their scores; the scores of both are
+        // within 2^-16 of themselves.  Neighbours that are further apart than this are in
+        // order, and with them all; equal logits are in any case.
+        double* by_rank = reinterpret_cast<double*>(s_cand[tok]);
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+          by_rank[rank[i]] = r[i];
+          sorted[rank[i]] = x[i];
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+          if (rank[i] + 1 < total && (some >> (lane & 48) & 0xffffu)) {
+            const float y = sorted[rank[i] + 1], s0 = score(x[i]), s1 = score(y);
+            const double tol = 0x1p-18 * (double)fabsf(s0 - s1) + 0x1p-33 * (double)(s0 + s1) +
+                               0x1p-50 * fabs(r[i]) + 0x1p-140;
+            unsure |= x[i] != y && !(r[i] - by_rank[rank[i] + 1] > tol);
+          }
+      }
     }
   }
 

@@ -152,6 +152,37 @@ def test_few_near_ties(k, device):
         _check(torch.from_numpy(lg), k, True, G, keep, "softmax", torch.from_numpy(bias / E))
 
 
+@pytest.mark.parametrize("k", [1, 8, 10, 16, 24])
+def test_few_near_ties_of_softmax(k, device):
+    """The same for softmax scores with a bias, whose sum over the experts moves with the
+    logit that is set: some rows a rounding of 32 bits apart, some of much less."""
+    banner(f"grouped_topk few near ties of softmax k={k}")
+    rng = np.random.default_rng(50 + k)
+    for E, G, keep in ((349, 1, 1), (64, 1, 1), (512, 2, 1), (512, 4, 3), (512, 8, 5), (256, 8, 4),
+                       (512, 16, 12)):
+        T = 120
+        lg = rng.standard_normal((T, E)).astype(np.float32)
+        bias = (0.3 / E * rng.standard_normal(E)).astype(np.float32)
+        for t in range(T):
+            e = np.exp(lg[t].astype(np.float64))
+            order = np.argsort(-(e / e.sum() + bias))
+            i = rng.integers(0, min(E - 2, k + 3))
+            a, b = order[i], order[i + 1 + int(rng.integers(0, 2))]
+            d = float(bias[b]) - float(bias[a])
+            # e_a / S + bias_a = y / S + bias_b with S = (sum of the others) + y
+            y = (e[a] - d * (e.sum() - e[b])) / (1 + d) * (1 + rng.integers(-3, 4) * 2.0 ** -22)
+            if y > 1e-3:
+                lg[t, b] = np.float32(np.log(y))
+        lg[0], lg[1, :] = lg[0, 0], lg[1, :1]           # (all equal: the bias decides)
+        lg[2, ::2] = lg[2, 1::2][:lg[2, ::2].size] if E % 2 == 0 else lg[2, ::2]
+        for rn in (True, False):
+            _check(torch.from_numpy(lg), k, rn, G, keep, "softmax", torch.from_numpy(bias))
+        flat = torch.zeros(E)                           # (equal logits tie: the lower id)
+        _check(torch.from_numpy(lg), k, True, G, keep, "softmax", flat)
+        _check(torch.from_numpy(lg).bfloat16(), k, True, G, keep, "softmax", flat)
+        _check(torch.from_numpy(lg * 60).float(), k, False, G, keep, "softmax", flat)
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 def test_masks(scoring, device):
     """-inf and NaN in logits and bias, rows and groups without an expert left, +inf,

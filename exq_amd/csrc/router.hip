@@ -403,7 +403,8 @@ __device__ __forceinline__ void rank_experts(const float (&key)[CH], int e0, int
 // Adding the bias rounds once.  A ranking between two values no further apart than this
 // is made in 64 bits (`tol`: 9 for sigmoid scores, 10 / S + 64 times the span of the biases
 // for softmax, a little over 2 |r| for the rounded sums): among the candidates where it
-// is theirs, by route_row otherwise.  A sum of two scores has twice the bound.  With
+// is theirs, by route_row otherwise.  A group's sum of two has twice the bound of the scores,
+// and the roundings of both addends.  With
 // logits as they come and a small bias that is one row in some thousands, but then most
 // batches have one, and the wave that does is the last to end: 4,096 tokens 12.7 us with
 // route_row alone.
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
       v2 = fmaxf(v2, fminf(v1, key[p]));
       v1 = fmaxf(v1, key[p]);
     }
-    float v;
+    float v, size;  // a group's value, and the size of what it is the sum of
     if (a.top2) {
       auto merge = [&](float o1, float o2) {
         v2 = fmaxf(fminf(v1, o1), fmaxf(v2, o2));
@@ -529,8 +530,10 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
       if constexpr (LG >= 8) merge(rowf<0x141>(v1), rowf<0x141>(v2));
       const float s1 = a.bias ? v1 : score(v1), s2 = a.bias ? v2 : score(v2);
       v = v1 > -INFINITY ? s1 + (v2 > -INFINITY ? s2 : 0.f) : -INFINITY;
+      size = fabsf(s1) + (v2 > -INFINITY ? fabsf(s2) : 0.f);
     } else {
       v = row_reduce<LG>(v1, max_op);
+      size = fabsf(v);
     }
     int before = 0;  // groups that come first
     unrolled<1, G>([&](auto j) {
@@ -541,10 +544,16 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
     });
     const bool keep = before < a.top_groups;
     if (a.bias || a.top2) {
-      const float worst = row_reduce<16>(keep ? v : INFINITY, min_op);
-      const float next = row_reduce<16>(keep ? -INFINITY : v, max_op);
-      const float tol = 2.f * tol0 + 0x1.2p-22f * fabsf(worst);
-      unsure = next > -INFINITY && !(worst - next > tol);
+      // `err`: how far v may be from its value in 64 bits, by the errors of its scores, the
+      // rounding of each addend at the addend's own size (opposed ones have a small sum and
+      // large roundings), and those of the sum and of v -+ err
+      const float err = tol0 + 0x1.2p-24f * size + 0x1.2p-23f * fabsf(v);
+      const bool known = err < INFINITY;
+      const float least = known ? v - err : -INFINITY;
+      const float most = known ? v + err : v > -INFINITY ? INFINITY : -INFINITY;
+      const float worst = row_reduce<16>(keep ? least : INFINITY, min_op);
+      const float next = row_reduce<16>(keep ? -INFINITY : most, max_op);
+      unsure = next > -INFINITY && !(worst > next);
     }
     // the kept groups, again over all lanes: lanes2 lanes for each of them
     float* keys = s_key[tok];

@@ -1,0 +1,46 @@
+"""grouped_topk where a group's value is small beside what it is the sum of, or past the
+largest float32: the order of the groups is that of the 64-bit oracle.
+
+Ids exactly.  The oracle and the kernel both rank in 64 bits, and what their scores may
+differ by (2^-52 of a score, rounded at the size of a bias of 1000: 2^-43) is far below the
+spacing of the values here (logits some 1e-6 apart)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import dense
+from tests._helpers import banner
+
+pytestmark = pytest.mark.gpu
+
+
+def _ids_match(logits, bias, k, G, keep, scoring, group_score="top2"):
+    from exq_amd.kernels import grouped_topk
+    _, ids = grouped_topk(torch.from_numpy(logits).cuda(), k, True, G, keep, scoring_func=scoring,
+                          correction_bias=torch.from_numpy(bias).cuda(), group_score=group_score)
+    want, _ = dense.grouped_topk(logits, k, True, G, keep, scoring, bias, group_score)
+    got = ids.cpu().numpy()
+    bad = np.flatnonzero((got != want).any(1))
+    assert bad.size == 0, f"{bad.size} of {len(got)} rows, first {got[bad[0]]}, not {want[bad[0]]}"
+
+
+@pytest.mark.parametrize("E,G,keep", [(8, 4, 2), (32, 2, 1), (64, 16, 5), (256, 8, 4), (512, 16, 7),
+                                      (30, 10, 4)])
+@pytest.mark.parametrize("size", [24.0, 1000.0])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_opposed_biases_in_a_group(E, G, keep, size, scoring, device):
+    """The two best experts of every group have biases of +size and -size, so the roundings of
+    their values are far larger than that of the sum of both."""
+    banner(f"grouped_topk opposed biases of {size} E={E} G={G} keep={keep} {scoring}")
+    rng = np.random.default_rng(E + G)
+    T, gs = 400, E // G
+    bias = np.full((G, gs), -2.0 * size)
+    for g in range(G):
+        hi, lo = rng.permutation(gs)[:2]
+        bias[g, hi], bias[g, lo] = size, -size
+    bias = bias.reshape(E).astype(np.float32)
+    for step in (2e-5, 2e-6):
+        lg = (rng.standard_normal((T, 1)) + step * rng.standard_normal((T, E))).astype(np.float32)
+        for k in (1, min(keep * gs, 2 * keep)):
+            _ids_match(lg, bias, k, G, keep, scoring)
+        _ids_match(lg, bias, 1, G, keep, scoring, "max")

@@ -548,9 +548,10 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
       // rounding of each addend at the addend's own size (opposed ones have a small sum and
       // large roundings), and those of the sum and of v -+ err
       const float err = tol0 + 0x1.2p-24f * size + 0x1.2p-23f * fabsf(v);
-      const bool known = err < INFINITY;
+      // (past the largest float, also below: then v may be -inf and the group not empty)
+      const bool known = err < INFINITY, empty = !((a.top2 ? v1 : v) > -INFINITY);
       const float least = known ? v - err : -INFINITY;
-      const float most = known ? v + err : v > -INFINITY ? INFINITY : -INFINITY;
+      const float most = known ? v + err : empty ? -INFINITY : INFINITY;
       const float worst = row_reduce<16>(keep ? least : INFINITY, min_op);
       const float next = row_reduce<16>(keep ? -INFINITY : most, max_op);
       unsure = next > -INFINITY && !(worst > next);

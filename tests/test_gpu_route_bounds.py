@@ -44,3 +44,26 @@ def test_opposed_biases_in_a_group(E, G, keep, size, scoring, device):
         for k in (1, min(keep * gs, 2 * keep)):
             _ids_match(lg, bias, k, G, keep, scoring)
         _ids_match(lg, bias, 1, G, keep, scoring, "max")
+
+
+@pytest.mark.parametrize("E,G,keep", [(16, 8, 5), (32, 16, 7), (16, 4, 2), (48, 2, 1), (24, 6, 4)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_sums_past_the_largest_float(E, G, keep, scoring, device):
+    """Sums of two biases beyond the range of float32, below and above, beside groups without
+    an expert: 64 bits hold them, and a group with an expert comes before one without."""
+    banner(f"grouped_topk sums past the largest float E={E} G={G} keep={keep} {scoring}")
+    rng = np.random.default_rng(E)
+    gs = E // G
+    for sign in (-1.0, 1.0):
+        for _ in range(20):
+            bias = np.full((G, gs), -np.inf)
+            bias[:, :2] = sign * rng.integers(20, 34, (G, 2)) * 1e37
+            lg = rng.standard_normal((8, G, gs))
+            lg[1:, 0] = -np.inf                         # no expert in the lowest groups
+            lg[2:, G // 2] = np.nan
+            lg[3:, 0, 0] = 0.0                          # (one)
+            _ids_match(lg.reshape(8, E).astype(np.float32), bias.reshape(E).astype(np.float32),
+                       2, G, keep, scoring)
+    bias = rng.permutation(np.linspace(-1, 1, E) * 3.4e38)
+    lg = rng.standard_normal((50, E)).astype(np.float32)
+    _ids_match(lg, bias.astype(np.float32), 2, G, keep, scoring)

@@ -237,11 +237,12 @@ __device__ void route_row(const RouteArgs& a, int64_t row, int lane, double* mem
   if (lane < a.k) store_choice(a, row, lane, my_id, w * a.scale);
 }
 
+constexpr int kRowsGrid = 1 << 23;  // work-groups in x: 2^32 threads are more than a launch takes
 template <int MAXC>
 __global__ void __launch_bounds__(256) route_rows_kernel(RouteArgs a) {
   __shared__ double s_mem[4][64 * MAXC];
   const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int row = (blockIdx.y * kRowsGrid + blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= a.T) return;  // (wave-uniform; the waves never meet)
   if (a.n_valid && row >= *a.n_valid) {
     if (lane < a.k) store_choice(a, row, lane, -1, 0.f);
@@ -728,7 +729,8 @@ int launch_tokens(const RouteArgs& a, hipStream_t s) {
   return check_launch("route_tokens_kernel");
 }
 int launch_rows(const RouteArgs& a, hipStream_t s) {
-  const dim3 g((unsigned)cdiv(a.T, 4));
+  const int64_t n = cdiv(a.T, 4);
+  const dim3 g((unsigned)(n < kRowsGrid ? n : kRowsGrid), (unsigned)cdiv(n, kRowsGrid));
   if (a.E <= 256)
     hipLaunchKernelGGL(route_rows_kernel<4>, g, dim3(256), 0, s, a);
   else

@@ -67,3 +67,17 @@ def test_sums_past_the_largest_float(E, G, keep, scoring, device):
     bias = rng.permutation(np.linspace(-1, 1, E) * 3.4e38)
     lg = rng.standard_normal((50, E)).astype(np.float32)
     _ids_match(lg, bias.astype(np.float32), 2, G, keep, scoring)
+
+
+def test_largest_token_count(device):
+    """The largest batch that the call takes, on the kernel with four rows a work-group."""
+    banner("grouped_topk 2^26 - 1 tokens")
+    from exq_amd.kernels import grouped_topk
+    T = (1 << 26) - 1
+    g = torch.Generator(device="cuda").manual_seed(3)
+    lg = torch.randint(-8, 9, (T, 3), generator=g, device="cuda", dtype=torch.int8).bfloat16()
+    w, ids = grouped_topk(lg, 1, True, 3, 2, weights_dtype=torch.bfloat16)
+    a, b, c = lg.unbind(1)
+    want = torch.where((a >= b) & (a >= c), 0, torch.where(b >= c, 1, 2))
+    assert torch.equal(ids[:, 0], want.int())
+    assert bool((w == 1).all())

@@ -69,6 +69,10 @@ __device__ __forceinline__ double wave_max64(double v) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
   return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
+// LDS that holds floats or candidates first and doubles later: accesses by this type are
+// ordered with all others.  Its arrays are declared 16-byte aligned.
+typedef double __attribute__((may_alias)) lds_double;
+
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
@@ -110,7 +114,7 @@ __device__ __forceinline__ float choice_weight(const RouteArgs& a, float x, floa
 // of the wave's own LDS.  The loops over c stay rolled where they hold an exponential:
 // as the rare part of route_tokens_kernel this runs from a cold instruction cache.
 template <int MAXC>
-__device__ void route_row(const RouteArgs& a, int64_t row, int lane, double* mem) {
+__device__ void route_row(const RouteArgs& a, int64_t row, int lane, lds_double* mem) {
   float b[MAXC];
   float m = -FLT_MAX;
 #pragma unroll
@@ -161,7 +165,7 @@ __device__ void route_row(const RouteArgs& a, int64_t row, int lane, double* mem
         v2 = fmax(v2, fmin(v1, x));
         v1 = fmax(v1, x);
       };
-      const double* at = mem + lane * a.gs;
+      const lds_double* at = mem + lane * a.gs;
       int i = 0;
       for (; i + 4 <= a.gs; i += 4) {  // (four reads in flight)
         const double x0 = at[i], x1 = at[i + 1], x2 = at[i + 2], x3 = at[i + 3];
@@ -420,9 +424,10 @@ template <int CH, int G, int KC, int MAXC>
 __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
   constexpr int LG = 16 / G;       // lanes of a group
   constexpr int KEYS = 16 * CH + 4;  // floats of a token's keys in LDS
-  __shared__ Candidate s_cand[16][16 * KC + 1];
+  __shared__ __align__(16) Candidate s_cand[16][16 * KC + 1];
   __shared__ float s_sorted[16][16 * KC + 1];
   __shared__ __align__(16) float s_key[16][KEYS];  // (route_row: 16 CH doubles a wave)
+  static_assert(4 * KEYS * sizeof(float) >= 16 * CH * sizeof(double) && KEYS % 4 == 0, "s_key");
   const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int tok = threadIdx.x >> 4;   // token of the work-group
   const int row0 = blockIdx.x * 16 + (threadIdx.x >> 6) * 4;  // first row of the wave
@@ -663,7 +668,8 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
         // values by that much of the difference of their scores; the scores of both are
         // within 2^-16 of themselves.  Neighbours that are further apart than this are in
         // order, and with them all; equal logits are in any case.
-        double* by_rank = reinterpret_cast<double*>(s_cand[tok]);
+        static_assert(sizeof(Candidate) == sizeof(double), "a double per slot");
+        lds_double* by_rank = reinterpret_cast<lds_double*>(s_cand[tok]);
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
           by_rank[rank[i]] = r[i];
@@ -717,7 +723,7 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
   for (int t = 0; t < 4; ++t)
     if (again >> (16 * t) & 0xffffu)  // (the keys of the wave's tokens are not needed any more)
       route_row<MAXC>(a, row0 + t, lane,
-                      reinterpret_cast<double*>(s_key[(threadIdx.x >> 6) * 4]));
+                      reinterpret_cast<lds_double*>(s_key[(threadIdx.x >> 6) * 4]));
 }
 
 // The fast kernel's sizes: 1, 2, 4, 8 or 16 groups, at most 32 experts a lane and 24

@@ -66,23 +66,23 @@ __device__ __forceinline__ void activate_run(float (&v)[CNT], int act) {
 // writes zeros and reads nothing.  Inline asm (it has no output register), as the
 // compiler puts a wait for all copies in flight before the next LDS read after its
 // own builtin, which ends the overlap that the stages are for; every copy here is
-// waited for by count (wait_vm) and, across waves, by a barrier.
+// waited for by count (wait_vm) and, across waves, by a barrier.  The LDS address is
+// an operand in m0, so the compiler knows that m0 changes here.
 typedef void __attribute__((address_space(3)))* lptr_t;
 __device__ __forceinline__ uint32_t lds_offset(const unsigned char* p) {
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)p);
 }
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t lds, int voff, int soff) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds),
-               "v"(voff), "s"(r), "s"(soff)
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"{m0}"(lds), "v"(voff),
+               "s"(r), "s"(soff)
                : "memory");
 #endif
 }
 // The same for four bytes a lane from anywhere.
 __device__ __forceinline__ void touch(const uint16_t* p, uint32_t lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(p)
-               : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" ::"{m0}"(lds), "v"(p) : "memory");
 #endif
 }
 constexpr int kOob = 0x7ffffff0;          // a voff past every resource

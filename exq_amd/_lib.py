@@ -12,6 +12,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB_PATH = Path(__file__).resolve().parent / "libexq_hip.so"
 _lock = threading.Lock()
@@ -165,6 +166,16 @@ def launch(entry, args: tuple, index: int, what: str) -> None:
     status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         check(status, what)
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raise if a tensor carries a forward-mode tangent (which no_grad does not turn off)."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{what} has no forward-mode derivative: call it with the primal "
+                             f"tensors (torch.autograd.forward_ad.unpack_dual)")
 
 
 def require_gpu(*tensors: torch.Tensor) -> torch.device:

@@ -240,7 +240,9 @@ def grouped_topk(gating_output: torch.Tensor, topk: int, renormalize: bool,
     float32.  Slots that no expert is left for get id -1, which the expert layers
     drop, and weight 0; so do all slots of the rows from ``num_token_non_padded``
     (int32, one element on the device) on, the padding of a captured batch.
-    Stream-ordered, graph-capturable, no workspace, no backward.
+    Stream-ordered, graph-capturable, no workspace.  There is no derivative: inputs that
+    require a gradient are refused unless gradients are off, and those with a forward-mode
+    tangent, which ``torch.no_grad`` leaves on.
     """
     p = _route_problem(
         gating_output.shape, gating_output.dtype,
@@ -253,6 +255,7 @@ def grouped_topk(gating_output: torch.Tensor, topk: int, renormalize: bool,
     if torch.is_grad_enabled() and (gating_output.requires_grad or (
             correction_bias is not None and correction_bias.requires_grad)):
         raise ValueError("grouped_topk has no backward: call it under torch.no_grad()")
+    _lib.refuse_tangents("grouped_topk", gating_output, correction_bias)
     g = gating_output if gating_output.is_contiguous() else gating_output.contiguous()
     dev = _lib.require_gpu(g, correction_bias, num_token_non_padded)
     T = p.n_tokens

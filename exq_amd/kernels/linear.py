@@ -118,6 +118,7 @@ def _call(x, weight, bias, activation, residual, out_dtype, out, gated, what):
                                     or (residual is not None and residual.requires_grad)
                                     or (out is not None and out.requires_grad)):
         raise ValueError(f"{what} has no backward: call it under torch.no_grad()")
+    _lib.refuse_tangents(what, x, weight, bias, residual, out)
     dev = x.get_device()
     if dev < 0:
         raise _lib.ExqError("exq_amd kernels need tensors on a HIP device (got CPU tensor)")
@@ -147,7 +148,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     Rows must be contiguous, row strides are free (column slices, expanded rows).
     ``out`` may be ``residual`` itself, to add in place, and must not overlap any
     other input.  Stream-ordered, graph-capturable, no workspace.  There is no
-    backward: inputs that require a gradient are refused unless gradients are off.
+    derivative: inputs that require a gradient are refused unless gradients are off, and
+    those with a forward-mode tangent, which ``torch.no_grad`` leaves on.
     """
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unsupported activation {activation!r}")

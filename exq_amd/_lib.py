@@ -80,6 +80,7 @@ _SIGNATURES = {
     "exq_topk_softmax": ([_P, _INT, _I64, _I64, _I64, _INT, _P, _INT, _P, _INT, _P], _INT),
     "exq_grouped_topk": ([C.POINTER(RouteProblem), _P, _P, _P, _P, _P, _P], _INT),
     "exq_linear": ([C.POINTER(LinearProblem), _P, _P, _P, _P, _P, _P], _INT),
+    "exq_linear_kernel": ([C.POINTER(LinearProblem), _P, _P], C.c_char_p),
     "exq_build_ends_from_slots": ([_P, _I64, _P, _I64, _I64, _P, _P, _P], _INT),
     "exq_dispatch": ([_P, _INT, _I64, _I64, _P, _P, _P, _P], _INT),
     "exq_gather_hidden": ([_P, _INT, _I64, _I64, _P, _I64, _I64, _P, _P], _INT),

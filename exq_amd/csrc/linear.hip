@@ -851,41 +851,51 @@ int pick_shape(int64_t tokens, int64_t rows, bool gated) {
   return best;
 }
 
-template <bool BF, bool GATED>
-int launch_linear(const LinArgs& a, hipStream_t s) {
-  const bool aligned = (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0 && a.ldx % 8 == 0 &&
-                       a.ldw % 8 == 0 && a.K % 8 == 0 && span_fits(256, a.ldx, a.K) &&
-                       span_fits(256, a.ldw, a.K);
-  if (aligned) {
-    const int shape = pick_shape(a.T, a.N * (GATED ? 2 : 1), GATED);
-    switch (shape) {
-      case 0: return launch_stream<BF, GATED, 1, 2, 8, 3>(a, s);
-      case 1: return launch_stream<BF, GATED, 2, 2, 8, 2>(a, s);
-      case 2: return launch_stream<BF, GATED, 4, 2, 4, 3>(a, s);
-      case 3: return launch_tile<BF, GATED, 2, 2, 1, 1, 4, 0, true>(a, s);
-      case 4: return launch_tile<BF, GATED, 2, 2, 1, 2, 6, 0, true>(a, s);
-      case 5: return launch_tile<BF, GATED, 2, 4, 2, 1, 4, 0, true>(a, s);
-      case 6: return launch_tile<BF, GATED, 2, 4, 2, 2, 3, 0, false>(a, s);
-      case 7: return launch_tile<BF, GATED, 2, 4, 3, 2, 2, 3, false>(a, s);
-      case 8: return launch_tile<BF, GATED, 2, 2, 4, 4, 2, 4, false>(a, s);
-      default:
-        if constexpr (!GATED) {
-          return shape == 9 ? launch_stream<BF, GATED, 1, 1, 16, 2>(a, s)
-                            : launch_stream<BF, GATED, 2, 1, 8, 3>(a, s);
-        }
-    }
-  }
-  const int64_t rows = a.N * (GATED ? 2 : 1);
+// The kernels by tokens x weight rows of a work-group: kShapes, then those of any layout.
+constexpr const char* kKernels[] = {
+    "stream 16x32",     "stream 32x32",     "stream 64x32",     "tile 64x64",
+    "tile 64x128",      "tile 128x128",     "tile 128x256",     "tile 192x256",
+    "tile 256x256",     "stream 16x16",     "stream 32x16",     "any stream 16x16",
+    "any stream 16x32", "any stream 32x32", "any tile 64x64",   "any tile 128x128",
+};
+
+int pick_kernel(const LinArgs& a, bool gated) {
+  const int64_t rows = a.N * (gated ? 2 : 1);
+  if ((((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0 && a.ldx % 8 == 0 && a.ldw % 8 == 0 &&
+      a.K % 8 == 0 && span_fits(256, a.ldx, a.K) && span_fits(256, a.ldw, a.K))
+    return pick_shape(a.T, rows, gated);
   // (16 rows a work-group while they fit one round: 7 tokens x 8801 x 1664 22.0 us, 32 rows
   // 29.6)
-  if constexpr (!GATED) {
-    if (a.T <= 16 && a.N <= 16 * kCus) return launch_stream_any<BF, GATED, 1, 1, 16, 4>(a, s);
+  if (a.T <= 16) return !gated && a.N <= 16 * kCus ? 11 : 12;
+  if (cdiv(a.T, 32) * cdiv(rows, 32) <= 2 * kCus) return 13;
+  return cdiv(a.T, 128) * cdiv(rows, 128) <= kCus ? 14 : 15;
+}
+
+template <bool BF, bool GATED>
+int launch_linear(const LinArgs& a, hipStream_t s) {
+  const int kernel = pick_kernel(a, GATED);
+  switch (kernel) {
+    case 0: return launch_stream<BF, GATED, 1, 2, 8, 3>(a, s);
+    case 1: return launch_stream<BF, GATED, 2, 2, 8, 2>(a, s);
+    case 2: return launch_stream<BF, GATED, 4, 2, 4, 3>(a, s);
+    case 3: return launch_tile<BF, GATED, 2, 2, 1, 1, 4, 0, true>(a, s);
+    case 4: return launch_tile<BF, GATED, 2, 2, 1, 2, 6, 0, true>(a, s);
+    case 5: return launch_tile<BF, GATED, 2, 4, 2, 1, 4, 0, true>(a, s);
+    case 6: return launch_tile<BF, GATED, 2, 4, 2, 2, 3, 0, false>(a, s);
+    case 7: return launch_tile<BF, GATED, 2, 4, 3, 2, 2, 3, false>(a, s);
+    case 8: return launch_tile<BF, GATED, 2, 2, 4, 4, 2, 4, false>(a, s);
+    case 12: return launch_stream_any<BF, GATED, 1, 2, 8, 4>(a, s);
+    case 13: return launch_stream_any<BF, GATED, 2, 2, 8, 2>(a, s);
+    case 14: return launch_tile_any<BF, GATED, 2, 2, 1, 1>(a, s);
+    case 15: return launch_tile_any<BF, GATED, 2, 2, 2, 2>(a, s);
+    default:
+      if constexpr (!GATED) {
+        if (kernel == 9) return launch_stream<BF, GATED, 1, 1, 16, 2>(a, s);
+        if (kernel == 10) return launch_stream<BF, GATED, 2, 1, 8, 3>(a, s);
+        if (kernel == 11) return launch_stream_any<BF, GATED, 1, 1, 16, 4>(a, s);
+      }
+      return EXQ_ERROR_UNSUPPORTED;  // (not reached: every kernel that is picked is above)
   }
-  if (a.T <= 16) return launch_stream_any<BF, GATED, 1, 2, 8, 4>(a, s);
-  if (cdiv(a.T, 32) * cdiv(rows, 32) <= 2 * kCus)
-    return launch_stream_any<BF, GATED, 2, 2, 8, 2>(a, s);
-  if (cdiv(a.T, 128) * cdiv(rows, 128) <= kCus) return launch_tile_any<BF, GATED, 2, 2, 1, 1>(a, s);
-  return launch_tile_any<BF, GATED, 2, 2, 2, 2>(a, s);
 }
 
 }  // namespace
@@ -893,8 +903,8 @@ int launch_linear(const LinArgs& a, hipStream_t s) {
 
 using namespace exq;
 
-extern "C" int exq_linear(const exq_linear_problem* p, const void* x, const void* weight,
-                          const void* bias, const void* residual, void* out, exq_stream stream) {
+namespace {
+int check_problem(const exq_linear_problem* p, const void* bias, const void* residual) {
   const char* fn = "exq_linear";
   EXQ_REQUIRE(p, "%s: null problem", fn);
   EXQ_REQUIRE(is_act_dtype(p->act_dtype), "%s: x and W must be f16 or bf16", fn);
@@ -914,6 +924,16 @@ extern "C" int exq_linear(const exq_linear_problem* p, const void* x, const void
   EXQ_REQUIRE(p->x_stride >= 0 && p->weight_stride >= 0 && p->residual_stride >= 0 &&
                   (T <= 1 || p->out_stride >= N),
               "%s: row strides must not be negative, and out's at least N", fn);
+  return EXQ_SUCCESS;
+}
+}  // namespace
+
+extern "C" int exq_linear(const exq_linear_problem* p, const void* x, const void* weight,
+                          const void* bias, const void* residual, void* out, exq_stream stream) {
+  const char* fn = "exq_linear";
+  const int status = check_problem(p, bias, residual);
+  if (status != EXQ_SUCCESS) return status;
+  const int64_t T = p->n_tokens, K = p->in_features, N = p->out_features;
   if (T == 0) return EXQ_SUCCESS;
   EXQ_REQUIRE(x && weight && out, "%s: null pointer", fn);
   LinArgs a;
@@ -942,4 +962,18 @@ extern "C" int exq_linear(const exq_linear_problem* p, const void* x, const void
   if (p->act_dtype == EXQ_DTYPE_BF16)
     return p->gated ? launch_linear<true, true>(a, s) : launch_linear<true, false>(a, s);
   return p->gated ? launch_linear<false, true>(a, s) : launch_linear<false, false>(a, s);
+}
+
+extern "C" const char* exq_linear_kernel(const exq_linear_problem* p, const void* x,
+                                         const void* weight) {
+  if (check_problem(p, nullptr, nullptr) != EXQ_SUCCESS || p->n_tokens == 0) return nullptr;
+  LinArgs a = {};
+  a.x = reinterpret_cast<const uint16_t*>(x);
+  a.w = reinterpret_cast<const uint16_t*>(weight);
+  a.ldx = p->x_stride;
+  a.ldw = p->weight_stride;
+  a.T = p->n_tokens;
+  a.N = p->out_features;
+  a.K = p->in_features;
+  return kKernels[pick_kernel(a, p->gated != 0)];
 }

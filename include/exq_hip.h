@@ -499,6 +499,15 @@ int exq_set_stage_events(void* const* events, int n_events);
 int exq_stream_read(const void* buf, int64_t bytes, uint32_t* sink, int64_t sink_words,
                     exq_stream stream);
 
+/*
+ * Measurement hook (no counterpart in the reference): the kernel that exq_linear takes
+ * for a problem with x and weight at these addresses, as tokens x weight rows of a
+ * work-group ("tile 128x256"; "any ..." for rows that are not 16-byte aligned).  Null for
+ * a problem without work or one that exq_linear refuses.  Launches nothing.
+ */
+const char* exq_linear_kernel(const exq_linear_problem* problem, const void* x,
+                              const void* weight);
+
 #ifdef __cplusplus
 }
 #endif

@@ -864,8 +864,13 @@ int pick_kernel(const LinArgs& a, bool gated) {
   if ((((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0 && a.ldx % 8 == 0 && a.ldw % 8 == 0 &&
       a.K % 8 == 0 && span_fits(256, a.ldx, a.K) && span_fits(256, a.ldw, a.K))
     return pick_shape(a.T, rows, gated);
-  // (16 rows a work-group while they fit one round: 7 tokens x 8801 x 1664 22.0 us, 32 rows
-  // 29.6)
+  // 16 rows a work-group while they fit one round: 7 tokens x 8801 x 1664 22.0 us, 32 rows
+  // 29.6.  32 x 32 streams while two rounds hold them, which is where they and the 64 x 64
+  // tiles meet (K = 1001, 2047, 4095: 256 tokens x 2048, two rounds, 11.7, 22.9, 40.9 us and
+  // 12.6, 21.9, 47.0; 300 x 2048 15.1, 30.8, 56.1 and 12.9, 22.4, 51.3; 100 x 2048 8.2, 14.1,
+  // 22.4 and 13.0, 22.3, 38.3); 128 x 128 tiles from more than one round of them (2048 x 2048,
+  // one round, 26.0, 54.7, 88.8 us and 64 x 64 27.4, 53.7, 99.6; 2048 x 2200 31.5, 57.2, 96.9
+  // and 36.6, 71.5, 130.6; 1500 x 2048 29.2, 53.4, 87.0 and 23.3, 42.2, 74.8).
   if (a.T <= 16) return !gated && a.N <= 16 * kCus ? 11 : 12;
   if (cdiv(a.T, 32) * cdiv(rows, 32) <= 2 * kCus) return 13;
   return cdiv(a.T, 128) * cdiv(rows, 128) <= kCus ? 14 : 15;

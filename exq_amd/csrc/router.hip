@@ -727,7 +727,17 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
 }
 
 // The fast kernel's sizes: 1, 2, 4, 8 or 16 groups, at most 32 experts a lane and 24
-// choices (32 slots hold them with room for near ones).
+// choices.  The threshold is the k + 1-th of 32 values, so the nearer k is to 32 the more
+// experts pass it, and a row with more of them than slots goes to route_row after it has
+// been through here: with 512 experts in one group no row at k = 16, 1 to 3 of 100 at
+// k = 20 and more than half at k = 24.  us, here / route_rows_kernel, softmax, one group:
+//               512 tokens x 256   4,096 x 256    4,096 x 512    16,384 x 256   16,384 x 512
+//     k = 16         8.8 /  9.0     8.8 / 14.3    11.2 /  26.2    13.5 / 37.6    24.9 /  85.7
+//     k = 20        15.8 /  9.9    22.2 / 16.3    30.6 /  31.0    27.4 / 44.5    44.6 / 101.8
+//     k = 22        31.0 / 10.4    37.7 / 18.0    51.7 /  33.9    46.0 / 47.9    73.4 / 109.5
+//     k = 24        40.6 / 10.9    41.1 / 18.8    56.3 /  35.6    70.5 / 50.2   123.0 / 115.6
+// One token: 8 and 8 to 10.  So past k = 20 this kernel is the slower one for most batches
+// between a few tokens and some ten thousand.
 template <int CH, int G, int KC>
 int launch_tokens(const RouteArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((route_tokens_kernel<CH, G, KC, CH / 4 < 1 ? 1 : CH / 4>),
@@ -745,6 +755,9 @@ int launch_rows(const RouteArgs& a, hipStream_t s) {
 }
 template <int CH, int G>
 int launch_slots(const RouteArgs& a, hipStream_t s) {
+  // 16 slots up to k = 10, 32 beyond: 4,096 tokens x 256 softmax, k = 8 6.3 us and 8.7, k = 9
+  // 6.4 and 8.7, k = 10 8.7 with 32 and 6.4 or 10.6 with 16, by whether a row has more; one
+  // token 5.4 and 7.8.
   if (a.k <= 10) return launch_tokens<CH, G, 1>(a, s);
   if (kHalfOnly<CH, G, 2> && a.chunk2 > CH / 2) return launch_rows(a, s);
   return launch_tokens<CH, G, 2>(a, s);

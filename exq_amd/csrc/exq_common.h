@@ -73,6 +73,15 @@ __device__ __forceinline__ uint32_t f32_to_f16_bits(float f) {
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
+// A wave's LDS operations are carried out in their order; the fences keep the compiler to
+// that order, which the barrier alone does not bind for accesses that it knows to be at
+// different addresses of one lane (slot r written, slot r + 1 read).  No instruction.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Load element i of a float-typed array of runtime dtype as fp32.
 __device__ __forceinline__ float load_as_f32(const void* p, int dtype, int64_t i) {
   if (dtype == EXQ_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];

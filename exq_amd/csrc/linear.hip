@@ -417,7 +417,9 @@ __device__ __forceinline__ void store_sums(const LinArgs& a, float* sums,
         *reinterpret_cast<float4*>(sums + r32 * pitch<NT>() + t * 32 + 2 * v + 4 * h) =
             float4{acc[u][t][v], acc[u][t][v + 1], acc[u][t][v + 2], acc[u][t][v + 3]};
     __builtin_amdgcn_sched_barrier(0);  // (a few sums at a time leave the accumulators)
+    wave_sync();
     finish_wave<GATED, NT>(a, sums, m0 + u * 32, n0, lane);
+    wave_sync();
     __builtin_amdgcn_sched_barrier(0);
   }
 }

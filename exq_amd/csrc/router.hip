@@ -117,6 +117,7 @@ template <int MAXC>
 __device__ void route_row(const RouteArgs& a, int64_t row, int lane, lds_double* mem) {
   float b[MAXC];
   float m = -FLT_MAX;
+  wave_sync();  // (mem: of the row before, or the keys)
 #pragma unroll
   for (int c = 0; c < MAXC; ++c) {  // mem: the logits, -inf where the expert is masked
     const int e = lane + 64 * c;
@@ -154,7 +155,7 @@ __device__ void route_row(const RouteArgs& a, int64_t row, int lane, lds_double*
       if (e < a.E && mem[e] > -INFINITY) mem[e] += (double)b[c];
     }
   }
-  __builtin_amdgcn_wave_barrier();  // (the wave's own LDS, in order)
+  wave_sync();
 
   uint64_t keep = ~0ull;
   if (a.top_groups < a.G) {
@@ -373,7 +374,7 @@ __device__ __forceinline__ void rank_experts(const float (&key)[CH], int e0, int
       if (at < 16 * KC) cand[at] = Candidate{key[p], e0 + p};
       ++at;
     }
-  __builtin_amdgcn_wave_barrier();  // (the wave's own LDS, in order)
+  wave_sync();
 #pragma unroll
   for (int i = 0; i < KC; ++i) {
     const int slot = i * 16 + l16;
@@ -583,7 +584,7 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
     int n2 = first2 >= a.gs ? 0 : a.gs - first2 < a.chunk2 ? a.gs - first2 : a.chunk2;
     if (j >= a.top_groups) n2 = 0;
     e0 = g2 * a.gs + first2;
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     auto deal = [&](auto& to, auto size) __attribute__((always_inline)) {
       constexpr int N = decltype(size)::value;
       if (CH <= 16 && a.vec) {
@@ -617,7 +618,7 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
     float* sorted = s_sorted[tok];
 #pragma unroll
     for (int i = 0; i < KC; ++i) sorted[rank[i]] = c[i].key;
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     bool close = false;
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
@@ -670,12 +671,13 @@ __global__ void __launch_bounds__(256, 3) route_tokens_kernel(RouteArgs a) {
         // order, and with them all; equal logits are in any case.
         static_assert(sizeof(Candidate) == sizeof(double), "a double per slot");
         lds_double* by_rank = reinterpret_cast<lds_double*>(s_cand[tok]);
+        wave_sync();  // (the candidates and `sorted` have been read)
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
           by_rank[rank[i]] = r[i];
           sorted[rank[i]] = x[i];
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
 #pragma unroll
         for (int i = 0; i < KC; ++i)
           if (rank[i] + 1 < total && (some >> (lane & 48) & 0xffffu)) {

@@ -48,8 +48,9 @@ def grouped_topk(logits, top_k, renormalize, n_groups=1, topk_group=1, scoring="
             kept = sorted(value, key=lambda g: (-value[g], g))[:topk_group]
             experts = [e for e in experts if int(e) // gs in kept]
         chosen = sorted(experts, key=lambda e: (-rank[e], e))[:top_k]
-        if renormalize:
-            w = np.exp(log_s[chosen] - log_s[chosen].max())
+        if renormalize:   # (a softmax's ratios are those of the logits, without its sum)
+            u = (l if scoring == "softmax" else log_s)[chosen]
+            w = np.exp(u - u.max())
             w = w / w.sum()
         else:
             w = s[chosen]

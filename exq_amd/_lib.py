@@ -102,6 +102,12 @@ _SIGNATURES = {
     "exq_pack_int4": ([_P, _INT, _I64, _I64, _I64, _P, _P, _P], _INT),
     "exq_quantize_int8": ([_P, _INT, _I64, _I64, _P, _P, _P], _INT),
     "exq_fake_quant": ([_P, _INT, _I64, _I64, _INT, _I64, _P, _P], _INT),
+    "exq_quantize_mxfp4": ([_P, _INT, _I64, _I64, _I64, _P, _P, _P], _INT),
+    "exq_dequantize_mxfp4": ([_P, _P, _I64, _I64, _P, _INT, _P], _INT),
+    "exq_tile_mxfp4": ([_P, _P, _I64, _I64, _I64, _INT, _P, _P, _P], _INT),
+    "exq_linear_mxfp4": ([C.POINTER(LinearProblem), _P, _P, _P, _P, _P, _P, _P, _P], _INT),
+    "exq_moe_mxfp4_workspace_size": ([C.POINTER(MoeProblem)], _SZ),
+    "exq_moe_mxfp4_forward": ([C.POINTER(MoeProblem), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P], _INT),
     "exq_stream_read": ([_P, _I64, _P, _I64, _P], _INT),
 }
 

@@ -18,7 +18,7 @@ BUILD = PKG / "_build"
 LIB = PKG / "libexq_hip.so"
 
 SOURCES = ["elementwise.hip", "routing.hip", "pack.hip", "moe_mfma.hip", "decode.hip", "prefill.hip", "rows.hip", "noalloc.hip",
-           "router.hip", "linear.hip"]
+           "router.hip", "linear.hip", "mxfp4_quant.hip", "mxfp4_linear.hip", "mxfp4_moe.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

@@ -5,23 +5,13 @@
 //
 // The weight rows are the MFMA's A operand and the tokens its B operand, so a lane
 // ends with four consecutive output columns of one token.
-#include "exq_internal.h"
+#include "lds_copy.h"
+#include "linear_epilogue.h"
 
 namespace exq {
 namespace {
 
-struct LinArgs {
-  const uint16_t* x;
-  const uint16_t* w;
-  const void* bias;   // [N] ([2N] gated) or null
-  const void* res;    // [T, N] or null
-  void* out;
-  int64_t ldx, ldw, ldr, ldo;  // elements from row to row
-  int64_t T, N, K;             // N: output columns
-  int bdt, rdt, odt, act;
-  int vec_b, vec_r, vec_o;     // four consecutive elements may be accessed at once
-  int odd;                     // rows of x or W may start at an odd 2-byte address
-};
+using namespace lin;
 
 template <bool BF>
 __device__ __forceinline__ f32x4_t mfma(const uint4& a, const uint4& b, f32x4_t c) {
@@ -34,71 +24,7 @@ __device__ __forceinline__ f32x4_t mfma(const uint4& a, const uint4& b, f32x4_t 
   }
 }
 
-// silu(v) = v / (1 + e^-v); sigmoid(v) = 1 / (1 + e^-v); gelu_tanh(v) = v / (1 + e^-z)
-// with z = 2 sqrt(2 / pi) (v + 0.044715 v^3), as (1 + tanh(z / 2)) / 2 = 1 / (1 + e^-z):
-// one exponential and one division serve all three.
-__device__ __forceinline__ float logistic_act(float v, int act) {
-  const float z = act == EXQ_ACT_GELU_TANH
-                      ? 1.5957691216057308f * (v + 0.044715f * v * v * v) : v;
-  return (act == EXQ_ACT_SIGMOID ? 1.f : v) / (1.f + expf(-z));
-}
-__device__ __forceinline__ float erf_gelu(float v) {
-  return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-}
-template <int CNT>
-__device__ __forceinline__ void activate_run(float (&v)[CNT], int act) {
-  if (act == EXQ_ACT_NONE) return;
-  if (act == EXQ_ACT_RELU) {
-#pragma unroll
-    for (int c = 0; c < CNT; ++c) v[c] = v[c] < 0.f ? 0.f : v[c];  // (NaN stays)
-  } else if (act == EXQ_ACT_GELU) {
-#pragma unroll
-    for (int c = 0; c < CNT; ++c) v[c] = erf_gelu(v[c]);
-  } else {
-#pragma unroll
-    for (int c = 0; c < CNT; ++c) v[c] = logistic_act(v[c], act);
-  }
-}
-
 // ---- aligned rows: copies straight into LDS ----------------------------------
-// 16 bytes per lane from buffer `r` at byte offset voff + soff into LDS at
-// lds + 16 * lane; `lds` and `soff` are wave-uniform.  A voff past the resource
-// writes zeros and reads nothing.  Inline asm (it has no output register), as the
-// compiler puts a wait for all copies in flight before the next LDS read after its
-// own builtin, which ends the overlap that the stages are for; every copy here is
-// waited for by count (wait_vm) and, across waves, by a barrier.  The LDS address is
-// an operand in m0, so the compiler knows that m0 changes here.
-typedef void __attribute__((address_space(3)))* lptr_t;
-__device__ __forceinline__ uint32_t lds_offset(const unsigned char* p) {
-  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)p);
-}
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t lds, int voff, int soff) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"{m0}"(lds), "v"(voff),
-               "s"(r), "s"(soff)
-               : "memory");
-#endif
-}
-// The same for four bytes a lane from anywhere.
-__device__ __forceinline__ void touch(const uint16_t* p, uint32_t lds) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" ::"{m0}"(lds), "v"(p) : "memory");
-#endif
-}
-constexpr int kOob = 0x7ffffff0;          // a voff past every resource
-constexpr int64_t kSpan = 0x7fffff00;     // bytes that one resource covers at most
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const uint16_t* base) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), (short)0, (int)kSpan,
-                                           0x00020000);
-}
-// LDS written by a copy is ordered only by the vmcnt wait, which the compiler does
-// not see as a dependency: volatile asm that no memory access moves across.
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-
 // LDS rows are 128 bytes (64 k), eight 16-byte columns; column c of row r holds the
 // row's chunk c ^ swz(r).  A ds_read_b128 is served 16 lanes at a time (equal bit 5
 // and equal parity of bits 2..4 of the lane id), 256 bytes a cycle; with lane
@@ -111,127 +37,6 @@ __device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
 template <int TILES>
 __device__ __forceinline__ int run_col(int t, int i) {
   return (i >> 2) * (4 * TILES) + t * 4 + (i & 3);
-}
-
-// CNT (a multiple of 4) consecutive values at element i.
-template <int CNT>
-__device__ __forceinline__ void load_run(const void* p, int dt, int64_t i, float (&v)[CNT]) {
-#pragma unroll
-  for (int c = 0; c < CNT; c += 4) {
-    if (dt == EXQ_DTYPE_F32) {
-      const float4 f = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i + c);
-      v[c] = f.x; v[c + 1] = f.y; v[c + 2] = f.z; v[c + 3] = f.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + i + c);
-      const bool bf = dt == EXQ_DTYPE_BF16;
-      v[c] = bf ? __uint_as_float(u.x << 16) : f16_bits_to_f32(u.x & 0xffffu);
-      v[c + 1] = bf ? __uint_as_float(u.x & 0xffff0000u) : f16_bits_to_f32(u.x >> 16);
-      v[c + 2] = bf ? __uint_as_float(u.y << 16) : f16_bits_to_f32(u.y & 0xffffu);
-      v[c + 3] = bf ? __uint_as_float(u.y & 0xffff0000u) : f16_bits_to_f32(u.y >> 16);
-    }
-  }
-}
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf) {
-  if (bf) {
-    bf16x2_t h;
-    h[0] = (__bf16)lo;
-    h[1] = (__bf16)hi;
-    return __builtin_bit_cast(uint32_t, h);
-  }
-  f16x2_t h;
-  h[0] = (_Float16)lo;
-  h[1] = (_Float16)hi;
-  return __builtin_bit_cast(uint32_t, h);
-}
-template <int CNT>
-__device__ __forceinline__ void store_run(void* p, int dt, int64_t i, const float (&v)[CNT]) {
-  if (dt == EXQ_DTYPE_F32) {
-#pragma unroll
-    for (int c = 0; c < CNT; c += 4)
-      *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i + c) =
-          float4{v[c], v[c + 1], v[c + 2], v[c + 3]};
-  } else {
-    uint16_t* o = reinterpret_cast<uint16_t*>(p) + i;
-    const bool bf = dt == EXQ_DTYPE_BF16;
-    uint32_t d[CNT / 2];
-#pragma unroll
-    for (int c = 0; c < CNT; c += 2) d[c / 2] = pack16(v[c], v[c + 1], bf);
-#pragma unroll
-    for (int c = 0; c < CNT / 2; c += 2)
-      *reinterpret_cast<uint2*>(o + 2 * c) = uint2{d[c], d[c + 1]};
-  }
-}
-// The epilogue of CNT consecutive columns n.. of token m, in two parts, so that the
-// residual of several runs can be on its way before the first is used.
-template <int CNT>
-__device__ __forceinline__ void fetch_residual(const LinArgs& a, int64_t m, int64_t n,
-                                               float (&r)[CNT]) {
-  if (!a.res || m >= a.T || n >= a.N) return;
-  if (n + CNT <= a.N && a.vec_r) {
-    load_run<CNT>(a.res, a.rdt, m * a.ldr + n, r);
-  } else {
-#pragma unroll
-    for (int c = 0; c < CNT; ++c)
-      r[c] = n + c < a.N ? load_as_f32(a.res, a.rdt, m * a.ldr + n + c) : 0.f;
-  }
-}
-template <int CNT>
-__device__ __forceinline__ void add_bias(const LinArgs& a, int64_t n, int64_t off, bool whole,
-                                         float (&y)[CNT]) {
-  float b[CNT];
-  if (whole && a.vec_b) {
-    load_run<CNT>(a.bias, a.bdt, off + n, b);
-  } else {
-#pragma unroll
-    for (int c = 0; c < CNT; ++c)
-      b[c] = n + c < a.N ? load_as_f32(a.bias, a.bdt, off + n + c) : 0.f;
-  }
-#pragma unroll
-  for (int c = 0; c < CNT; ++c) y[c] += b[c];
-}
-template <int CNT, bool GATED>
-__device__ __forceinline__ void finish_run(const LinArgs& a, int64_t m, int64_t n, float (&y)[CNT],
-                                           float (&u)[CNT], const float (&r)[CNT]) {
-  if (m >= a.T || n >= a.N) return;
-  const bool whole = n + CNT <= a.N;
-  if (a.bias) {
-    add_bias<CNT>(a, n, 0, whole, y);
-    if constexpr (GATED) add_bias<CNT>(a, n, a.N, whole, u);
-  }
-  activate_run<CNT>(y, a.act);
-  if constexpr (GATED) {
-#pragma unroll
-    for (int c = 0; c < CNT; ++c) y[c] *= u[c];
-  } else if (a.res) {
-#pragma unroll
-    for (int c = 0; c < CNT; ++c) y[c] += r[c];
-  }
-  if (whole && a.vec_o) {
-    store_run<CNT>(a.out, a.odt, m * a.ldo + n, y);
-  } else {
-#pragma unroll
-    for (int c = 0; c < CNT; ++c)
-      if (n + c < a.N) store_from_f32(a.out, a.odt, m * a.ldo + n + c, y[c]);
-  }
-}
-
-// Unit (token block mt of nm, column block nt of nn) of work-group bid: work-group i
-// runs on XCD i % 8, and each XCD takes an eighth of the units in a row, the token
-// blocks fastest in groups of GM, so that what runs together shares rows of both
-// operands in that XCD's L2.  False: none.
-template <int GM>
-__device__ __forceinline__ bool unit_of(int bid, int nm, int nn, int& mt, int& nt) {
-  const int U = nm * nn;
-  const int per = (U + 7) >> 3;
-  const int local = bid >> 3;
-  const int v = (bid & 7) * per + local;
-  if (local >= per || v >= U) return false;
-  const int g = v / (GM * nn), first = g * GM;
-  const int size = nm - first < GM ? nm - first : GM;
-  const int rem = v - g * GM * nn;
-  nt = rem / size;
-  mt = first + rem - nt * size;
-  return true;
 }
 
 // The sums of W waves over their parts of the contraction, joined through LDS in wave

@@ -12,6 +12,8 @@ from .moe_int4_kernel import (moe_int4_forward, moe_int4_full_forward, pack_expe
 from . import exq_dispatch
 from .exq_dispatch import fused_topk, grouped_topk
 from .linear import fused_gated_linear, fused_linear
+from .mxfp4 import (Mxfp4Weight, dequantize_mxfp4, fused_experts_mxfp4,
+                    fused_gated_linear_mxfp4, fused_linear_mxfp4, quantize_mxfp4)
 from .quant_shim import quantize_tensor_int4, quantize_tensor_int8
 
 __all__ = [
@@ -33,6 +35,12 @@ __all__ = [
     "grouped_topk",
     "fused_linear",
     "fused_gated_linear",
+    "Mxfp4Weight",
+    "quantize_mxfp4",
+    "dequantize_mxfp4",
+    "fused_linear_mxfp4",
+    "fused_gated_linear_mxfp4",
+    "fused_experts_mxfp4",
     "quantize_tensor_int4",
     "quantize_tensor_int8",
 ]

@@ -316,6 +316,58 @@ typedef struct exq_linear_problem {
 int exq_linear(const exq_linear_problem* problem, const void* x, const void* weight,
                const void* bias, const void* residual, void* out, exq_stream stream);
 
+/* ---- MXFP4 ---------------------------------------------------------------- */
+
+/*
+ * Microscaled 4-bit floating point (OCP MX, no counterpart in the reference): blocks
+ * of 32 values along a row share a scale 2^(s - 127), s one byte (255: NaN); a value
+ * is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.
+ *   packed [.., K/2] u8: two codes a byte, the even column in the low half
+ *   scales [.., K/32] u8
+ * K is a multiple of 32.  The products take a weight [rows, K] in the order of their
+ * tiles (exq_tile_mxfp4), with RT = ceil(rows / 16) (gated: 2 ceil(rows / 2 / 16), gate
+ * and up tiles in turn) and KB = ceil(K / 128), padding filled with zeros:
+ *   tiles       [RT, KB, 64, 16] u8: [rt, kb, 16 q + r, b] is byte b of the block
+ *               4 kb + q of row 16 rt + r (of its half)
+ *   tile_scales [RT, ceil(KB / 4), 64, 4] u8: [rt, g, 16 q + r, i] is the scale of the
+ *               block 4 (4 g + i) + q of that row
+ */
+
+/*
+ * Rows [rows, K] of x (f32 | f16 | bf16, x_stride elements apart, contiguous in
+ * themselves) to packed and scales.  With a the block's largest magnitude, s =
+ * floor(log2 a) - 2 + 127, at least 0, and each x / 2^(s - 127) goes to the nearest
+ * value, halfway to the even code, past 6 to 6; the sign of a zero stays.  A block with
+ * an infinity or a NaN gets the scale 255 and codes 0: it reads back as NaN.
+ */
+int exq_quantize_mxfp4(const void* x, int dtype, int64_t rows, int64_t K, int64_t x_stride,
+                       uint8_t* packed, uint8_t* scales, exq_stream stream);
+
+/*
+ * And back: out [rows, K] (f32 | f16 | bf16), rounded to nearest where the type cannot
+ * hold a value (bf16 holds all but 6 * 2^127 and 4 * 2^127, which become infinite).
+ */
+int exq_dequantize_mxfp4(const uint8_t* packed, const uint8_t* scales, int64_t rows, int64_t K,
+                         void* out, int dtype, exq_stream stream);
+
+/* packed [n_matrices, rows, K/2] and scales to tiles and tile_scales, each matrix alone. */
+int exq_tile_mxfp4(const uint8_t* packed, const uint8_t* scales, int64_t n_matrices,
+                   int64_t rows, int64_t K, int gated, uint8_t* tiles, uint8_t* tile_scales,
+                   exq_stream stream);
+
+/*
+ * exq_linear with an MXFP4 weight (its weight_stride is not read).  act_dtype f16 | bf16:
+ * x [T, K] is 16-bit and the weight's values take its type, exact in bf16, rounded to
+ * nearest in f16 (exact for scales 2^-23 .. 2^13); x_scales is not read.  act_dtype u8: x
+ * [T, K/2] is MXFP4 too, x_stride bytes from row to row, with x_scales [T, K/32].
+ * Products are summed in fp32 and the result is rounded once, to out_dtype.  x's rows,
+ * tiles and tile_scales are 16-byte aligned.  out may be residual itself (same pointer,
+ * dtype and stride) and must not overlap any other input.  No workspace.
+ */
+int exq_linear_mxfp4(const exq_linear_problem* problem, const void* x, const uint8_t* x_scales,
+                     const uint8_t* tiles, const uint8_t* tile_scales, const void* bias,
+                     const void* residual, void* out, exq_stream stream);
+
 /* ---- weight quantisation -------------------------------------------------- */
 
 /*
@@ -446,6 +498,23 @@ int exq_moe_mixed_forward(const exq_moe_problem* problem, const void* hidden,
                           const void* topk_ids, const void* topk_weights,
                           const exq_expert_bank* bank, void* out,
                           int64_t* sort_order_out, int32_t* expert_ends_out,
+                          void* workspace, size_t workspace_bytes, exq_stream stream);
+
+/*
+ * The MoE layer with MXFP4 experts: out[t] = sum_j w[t, j] * W2 (silu(Wg x_t) * Wu x_t)
+ * of expert ids[t, j], ids outside [0, n_experts) dropped (a token without experts gets
+ * zeros).  w13 [E, 2I, H] gated and w2 [E, H, I] in the order of tiles; weight values
+ * take hidden's type as in exq_linear_mxfp4, silu(gate) * up is rounded to it, sums are
+ * in fp32, and the k results of a token are added in a fixed order.  H and I are
+ * multiples of 32, n_experts <= 1024, top_k <= 64, at most 2^24 slots; group_size is 32
+ * and n_shared 0.  Pointers are 16-byte aligned.  The workspace needs no fill and must
+ * not be shared by calls that may run concurrently.  No counterpart in the reference.
+ */
+size_t exq_moe_mxfp4_workspace_size(const exq_moe_problem* problem);
+int exq_moe_mxfp4_forward(const exq_moe_problem* problem, const void* hidden,
+                          const void* topk_ids, const void* topk_weights,
+                          const uint8_t* w13_tiles, const uint8_t* w13_tile_scales,
+                          const uint8_t* w2_tiles, const uint8_t* w2_tile_scales, void* out,
                           void* workspace, size_t workspace_bytes, exq_stream stream);
 
 /*

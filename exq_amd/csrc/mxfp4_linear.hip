@@ -6,8 +6,10 @@
 //
 // Weight rows are the matrix instruction's A operand and tokens its B operand: lane (r, q)
 // ends with columns 4 q .. 4 q + 3 of a tile for token r.
-#include "linear_epilogue.h"
-#include "mxfp4.h"
+#include "mxfp4_tile.h"
+
+#include <stdlib.h>
+#include <type_traits>
 
 namespace exq {
 namespace {
@@ -80,8 +82,78 @@ __global__ void __launch_bounds__(256) mx_simple_kernel(MxArgs a, int nm, int nn
   finish_run<4, GATED>(a, mo, n, y, u, res);
 }
 
+// ---- many tokens: tiles -------------------------------------------------------------------
+template <bool BF, bool X4, bool GATED, int WM, int WN, int MT, int NT, int P>
+__global__ void __launch_bounds__(64 * WM * WN, MT == 8 ? 1 : X4 ? 2 : 3) mx_tile_kernel(MxArgs a, int nm, int nn) {
+  using T = std::conditional_t<X4, Tile4<WM, WN, MT, NT>, Tile16<BF, WM, WN, MT, NT, P>>;
+  constexpr int COLS = (GATED ? 8 : 16) * NT;      // output columns of a wave
+  constexpr int SUMS = T::W * wave_floats<NT>() * 4;
+  constexpr int LDS = T::LDS > SUMS ? T::LDS : SUMS;
+  __shared__ __align__(1024) unsigned char lds[LDS];
+  int mb, nb;
+  if (!unit_of<8>(blockIdx.x, nm, nn, mb, nb)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int64_t m0 = (int64_t)mb * T::BM, n0 = (int64_t)nb * COLS * WN;
+  const int rows = (int)(GATED ? (a.N + 15) / 16 * 2 : (a.N + 15) / 16);
+  int vo[T::D], rt[NT];
+#pragma unroll
+  for (int j = 0; j < T::D; ++j) {
+    const int r = T::row(wave, lane, j);
+    vo[j] = m0 + r < a.T ? (int)(r * a.ldx * (X4 ? 1 : 2) + T::piece(wave, lane) * 16) : kOob;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {   // (tiles past the last repeat it: what they give is not stored)
+    const int i = (nb * WN + wn) * NT + t;
+    rt[t] = i < rows ? i : rows - 1;
+  }
+  const int blocks = (int)(a.K / kBlock);
+  f32x4_t acc[MT][NT] = {};
+  if constexpr (X4) {
+    const uint8_t* x = reinterpret_cast<const uint8_t*>(a.x);
+    const uint8_t* xs[MT];
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      const int64_t m = m0 + (wm * MT + u) * 16 + (lane & 15);
+      xs[u] = a.xs + (m < a.T ? m : a.T - 1) * blocks;
+    }
+    T::run(lds, uniform_rsrc(x + m0 * a.ldx), vo, xs, a.tiles,
+           a.wscales, rt, a.KB, a.G, blocks, wave, lane, acc);
+  } else {
+    T::run(lds, uniform_rsrc(a.x + m0 * a.ldx), vo, a.tiles, a.wscales, rt, a.KB, a.G, blocks * 4,
+           wave, lane, acc);
+  }
+  const int64_t mw = m0 + wm * MT * 16, nw = n0 + wn * COLS;
+  emit_tiles<GATED, MT, NT>(reinterpret_cast<float*>(lds) + wave * wave_floats<NT>(), acc, lane,
+                            [&](int m, int c, float (&y)[8], float (&up)[8]) {
+                              float r[8];
+                              if constexpr (!GATED) fetch_residual<8>(a, mw + m, nw + c, r);
+                              finish_run<8, GATED>(a, mw + m, nw + c, y, up, r);
+                            });
+}
+
+template <bool BF, bool X4, bool GATED, int WM, int WN, int MT, int NT, int P>
+int launch_tile(const MxArgs& a, hipStream_t s) {
+  const int64_t nm = cdiv(a.T, 16 * MT * WM), nn = cdiv(a.N, (GATED ? 8 : 16) * NT * WN);
+  const int64_t grid = cdiv(nm * nn, 8) * 8;
+  EXQ_REQUIRE_SUPPORTED(grid * 64 * WM * WN < ((int64_t)1 << 32),
+                        "exq_linear_mxfp4: T=%lld x N=%lld is too large", (long long)a.T,
+                        (long long)a.N);
+  hipLaunchKernelGGL((mx_tile_kernel<BF, X4, GATED, WM, WN, MT, NT, P>), dim3((unsigned)grid),
+                     dim3(64 * WM * WN), 0, s, a, (int)nm, (int)nn);
+  return check_launch("mx_tile_kernel");
+}
+
 template <bool BF, bool X4, bool GATED>
 int launch_products(const MxArgs& a, hipStream_t s) {
+  const char* v = getenv("MXV");
+  if constexpr (X4) if (v && v[0] == '0') return launch_tile<BF, X4, GATED, 2, 2, 8, 8, 2>(a, s);
+  if (v && v[0] == '1') return launch_tile<BF, X4, GATED, 1, 4, 8, 4, 2>(a, s);
+  if (v && v[0] == '2') return launch_tile<BF, X4, GATED, 1, 4, 4, 4, 3>(a, s);
+  if (v && v[0] == '3') return launch_tile<BF, X4, GATED, 1, 4, 4, 2, 3>(a, s);
+  if (v && v[0] == '4') return launch_tile<BF, X4, GATED, 1, 4, 2, 2, 6>(a, s);
+  if (v && v[0] == '5') return launch_tile<BF, X4, GATED, 1, 4, 2, 4, 5>(a, s);
+  if (v && v[0] == '6') return launch_tile<BF, X4, GATED, 1, 4, 4, 4, 2>(a, s);
   const int64_t nm = cdiv(a.T, 16), nn = cdiv(a.N, 16), grid = cdiv(nm * nn, 4);
   EXQ_REQUIRE_SUPPORTED(grid * 256 < ((int64_t)1 << 32),
                         "exq_linear_mxfp4: T=%lld x N=%lld is too large", (long long)a.T,

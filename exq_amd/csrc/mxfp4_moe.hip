@@ -1,20 +1,17 @@
 // mxfp4_moe.hip -- the MoE layer with MXFP4 experts:
 //   out[t] = sum_j w[t, j] * W2_e (silu(Wg_e x_t) * (Wu_e x_t)),  e = ids[t, j]
+#include "mxfp4_route.h"
 #include "mxfp4_stream.h"
-
-#include <stdlib.h>
 
 namespace exq {
 namespace {
 
 using namespace mx;
 
-constexpr int kGroup = 16;  // rows of a token group
-
 struct MoeArgs {
-  const int* hdr;            // [0]: token groups
-  const TgEntry* tg;
-  const int* sorted;         // expert-sorted position -> slot
+  int* hdr;                  // [0]: token groups
+  TgEntry* tg;
+  int* sorted;         // expert-sorted position -> slot
   const uint16_t* x;         // gate/up: hidden [T, H]; down: mid [n, I]
   const uint4* tiles;        // [E, RT, KB]
   const uint32_t* wscales;   // [E, RT, G]
@@ -23,51 +20,7 @@ struct MoeArgs {
   float* part;               // [slots, H]
 };
 
-// One wave: a token group x a tile of rows.
-template <bool BF, bool GATEUP>
-__global__ void __launch_bounds__(256) moe_simple_kernel(MoeArgs a) {
-  constexpr int NT = GATEUP ? 2 : 1;
-  const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
-  if ((int)blockIdx.y >= a.hdr[0]) return;
-  const TgEntry g = a.tg[blockIdx.y];
-  const int nb = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (nb * NT >= a.RT) return;
-  const int pos = g.pos0 + (r16 < g.cnt ? r16 : 0);
-  const int slot = a.sorted[pos];
-  const uint16_t* x = a.x + (int64_t)(GATEUP ? slot / a.top_k : pos) * a.K;
-  const int blocks = a.K / kBlock;
-  f32x4_t acc[NT] = {};
-  for (int kb = 0; kb < a.KB; ++kb) {
-    const int b = kb * 4 + q;
-    uint4 xv[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      xv[j] = b < blocks ? *reinterpret_cast<const uint4*>(x + b * 32 + j * 8)
-                         : uint4{0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int64_t rt = (int64_t)g.e * a.RT + nb * NT + t;
-      const uint4 w = a.tiles[(rt * a.KB + kb) * 64 + lane];
-      const float s = __uint_as_float(
-          (a.wscales[(rt * a.G + (kb >> 2)) * 64 + lane] >> (8 * (kb & 3)) & 0xff) << 23);
-      const uint32_t c[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[t] = dev::dmfma<BF>(decode8<BF>(c[j], s), xv[j], acc[t]);
-    }
-  }
-  if (r16 >= g.cnt) return;
-#pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    const int n = nb * 16 + q * 4 + v;
-    if (n >= a.N) break;
-    if constexpr (GATEUP)  // (rounded to the activations' type: the next product's operand)
-      a.mid[(int64_t)pos * a.N + n] = (uint16_t)dev::to_act_bits<BF>(silu_f32(acc[0][v]) * acc[NT - 1][v]);
-    else
-      a.part[(int64_t)slot * a.N + n] = acc[0][v];
-  }
-}
-
-// ---- many tokens: tiles -------------------------------------------------------------------
+// ---- tiles ----------------------------------------------------------------------------------
 // Token groups of up to 64 expert-sorted rows x 64 NT weight rows: as many tokens as the
 // group has, by halves, and the fewer they are the more stages are on their way.
 constexpr int kTileGroup = 64;
@@ -90,7 +43,7 @@ inline int64_t spread_grid(int64_t n, int64_t n_tiles) {
 
 template <bool BF, bool GATEUP, int NT, int MT, int P>
 __device__ __forceinline__ void moe_tile(const MoeArgs& a, unsigned char* lds, const TgEntry& g,
-                                         int nb, int wave, int lane) {
+                                         const int* tokens, int nb, int wave, int lane) {
   using T = Tile16<BF, 1, 4, MT, NT, P>;
   constexpr int COLS = (GATEUP ? 8 : 16) * NT;     // result columns of a wave
   static_assert(T::LDS <= kTileLds && T::W * wave_floats<NT>() * 4 <= kTileLds, "LDS");
@@ -100,7 +53,7 @@ __device__ __forceinline__ void moe_tile(const MoeArgs& a, unsigned char* lds, c
   for (int j = 0; j < T::D; ++j) {
     const int r = T::row(wave, lane, j);
     if (r >= g.cnt) vo[j] = kOob;
-    else if (GATEUP) vo[j] = (a.sorted[g.pos0 + r] / a.top_k) * (a.K * 2) + pc * 16;
+    else if (GATEUP) vo[j] = (tokens ? tokens[r] : a.sorted[g.pos0 + r] / a.top_k) * (a.K * 2) + pc * 16;
     else vo[j] = r * (a.K * 2) + pc * 16;
   }
 #pragma unroll
@@ -132,17 +85,34 @@ __device__ __forceinline__ void moe_tile(const MoeArgs& a, unsigned char* lds, c
       });
 }
 
-template <bool BF, bool GATEUP, int NT>
-__global__ void __launch_bounds__(256, 3) moe_tile_kernel(MoeArgs a, int n_tiles) {
+// NSEG > 0: the kernel routes (gate/up), the plan in groups of PLAN rows.
+template <bool BF, bool GATEUP, int NT, int NSEG, int PLAN>
+__global__ void __launch_bounds__(256, 3) moe_tile_kernel(MoeArgs a, RouteArgs ra, int n_tiles) {
   __shared__ __align__(1024) unsigned char lds[kTileLds];
   int tgi, nb;
-  if (!spread_unit(blockIdx.x, a.hdr[0], n_tiles, tgi, nb)) return;
+  TgEntry at;
+  const int* tokens = nullptr;
+  if constexpr (NSEG > 0) {
+    using R = Router<NSEG>;
+    __shared__ TgEntry own;
+    __shared__ int rows[kTileGroup];
+    static_assert(R::kWords * 4 <= kTileLds && kTileGroup == 64, "routing scratch");
+    if (!R::template here<PLAN>(ra, reinterpret_cast<uint32_t*>(lds), &own, rows, [&](int n) {
+          return spread_unit(blockIdx.x, n, n_tiles, tgi, nb) ? tgi : -1;
+        }))
+      return;
+    at = own;
+    tokens = rows;
+  } else {
+    if (!spread_unit(blockIdx.x, a.hdr[0], n_tiles, tgi, nb)) return;
+    at = a.tg[tgi];
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const TgEntry at = a.tg[tgi];
   const TgEntry g{__builtin_amdgcn_readfirstlane(at.e), __builtin_amdgcn_readfirstlane(at.pos0),
                   __builtin_amdgcn_readfirstlane(at.cnt), 2};
-  if (g.cnt > 32) moe_tile<BF, GATEUP, NT, 4, 3>(a, lds, g, nb, wave, lane);
-  else moe_tile<BF, GATEUP, NT, 2, NT == 2 ? 5 : 4>(a, lds, g, nb, wave, lane);
+  if (g.cnt > 32) moe_tile<BF, GATEUP, NT, 4, 3>(a, lds, g, tokens, nb, wave, lane);
+  else if (g.cnt > 16) moe_tile<BF, GATEUP, NT, 2, NT == 4 ? 4 : 5>(a, lds, g, tokens, nb, wave, lane);
+  else moe_tile<BF, GATEUP, NT, 1, NT == 4 ? 5 : 8>(a, lds, g, tokens, nb, wave, lane);
 }
 
 // CPL columns a lane, eight slots' ids, weights and then rows in flight.  Bound: bytes, or
@@ -189,12 +159,75 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const float* part, con
     *reinterpret_cast<uint2*>(out + t * H + h) = uint2{d[0], d[CPL / 2 - 1]};
 }
 
+// Weight tiles of a wave: four (a work-group 256 weight rows), as its tokens are read least
+// so, fewer where the work-groups would not fill the CUs twice.
+int wave_tiles(int64_t groups, int64_t RT, int least) {
+  constexpr int64_t kFull = 512;
+  for (int nt = 4; nt > least; nt /= 2)
+    if (groups * cdiv(RT, 4 * nt) >= kFull) return nt;
+  return least;
+}
+template <typename Kernel>
+int launch_moe_tile(Kernel kernel, const MoeArgs& a, const RouteArgs& ra, int64_t groups, int nt,
+                    hipStream_t s) {
+  const int64_t n_tiles = cdiv(a.RT, 4 * nt), grid = spread_grid(groups, n_tiles);
+  EXQ_REQUIRE_SUPPORTED(grid * 256 < ((int64_t)1 << 32),
+                        "exq_moe_mxfp4_forward: %lld token groups x %d rows are too many",
+                        (long long)groups, a.RT * 16);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, s, a, ra, (int)n_tiles);
+  return check_launch("moe_tile_kernel");
+}
+template <bool BF, int NSEG, int PLAN>
+int launch_gateup_as(const MoeArgs& a, const RouteArgs& ra, hipStream_t s) {
+  const int64_t groups = tg_capacity(ra.n, ra.E, kTileGroup);
+  if (wave_tiles(groups, a.RT, 2) == 4)
+    return launch_moe_tile(moe_tile_kernel<BF, true, 4, NSEG, PLAN>, a, ra, groups, 4, s);
+  return launch_moe_tile(moe_tile_kernel<BF, true, 2, NSEG, PLAN>, a, ra, groups, 2, s);
+}
+template <bool BF>
+int launch_down(const MoeArgs& a, int64_t groups, hipStream_t s) {
+  switch (wave_tiles(groups, a.RT, 1)) {
+    case 4: return launch_moe_tile(moe_tile_kernel<BF, false, 4, 0, 64>, a, RouteArgs{}, groups, 4, s);
+    case 2: return launch_moe_tile(moe_tile_kernel<BF, false, 2, 0, 64>, a, RouteArgs{}, groups, 2, s);
+    default: return launch_moe_tile(moe_tile_kernel<BF, false, 1, 0, 64>, a, RouteArgs{}, groups, 1, s);
+  }
+}
+
+// How a batch runs: which kernels route, make the partial rows and add them.
+struct Path {
+  int64_t n;       // slots
+  bool by_slot;    // gate/up by slots, no routing
+  bool owned;      // down by output columns, no partial rows
+  int nseg;        // the gate/up tiles route, 64 nseg slots at most; 0: a plan kernel first
+};
+Path path_of(const exq_moe_problem* p) {
+  static_assert(kSlotSlots <= kOwnedSlots && kOwnedSlots <= 64, "paths");
+  Path r;
+  r.n = p->n_tokens * p->top_k;
+  r.owned = r.n <= kOwnedSlots;
+  r.by_slot = r.n <= kSlotSlots;
+  r.nseg = r.by_slot ? 0 : r.n <= 64 ? 1 : r.n <= 128 ? 2
+           : r.n <= 512 && p->n_experts <= Router<8>::kExperts ? 8 : 0;
+  return r;
+}
+
+template <bool BF>
+int launch_gateup(const MoeArgs& a, const RouteArgs& ra, const Path& r, hipStream_t s) {
+  if (r.owned) return launch_gateup_as<BF, 1, 16>(a, ra, s);   // (owned slots fit one segment)
+  switch (r.nseg) {
+    case 1: return launch_gateup_as<BF, 1, 64>(a, ra, s);
+    case 2: return launch_gateup_as<BF, 2, 64>(a, ra, s);
+    case 8: return launch_gateup_as<BF, 8, 64>(a, ra, s);
+    default: return launch_gateup_as<BF, 0, 64>(a, ra, s);
+  }
+}
+
 struct Layout {
   size_t hdr, tg, sorted, ends, blk, mid, part, total;
   int64_t tg_cap;
 };
 Layout layout(const exq_moe_problem* p) {
-  const int64_t n = p->n_tokens * p->top_k;
+  const Path r = path_of(p);
   Layout l;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -202,14 +235,14 @@ Layout layout(const exq_moe_problem* p) {
     at = align_up(at + bytes, 256);
     return o;
   };
-  l.tg_cap = tg_capacity(n, p->n_experts, kGroup);
+  l.tg_cap = tg_capacity(r.n, p->n_experts, r.owned ? 16 : kTileGroup);
   l.hdr = take(64);
   l.tg = take((size_t)l.tg_cap * sizeof(TgEntry));
-  l.sorted = take((size_t)n * 4);
+  l.sorted = take((size_t)r.n * 4);
   l.ends = take((size_t)(p->n_experts + 1) * 4);
-  l.blk = take((size_t)route_plan_blocks(n) * p->n_experts * 4);
-  l.mid = take((size_t)n * p->inter_size * 2);
-  l.part = take((size_t)n * p->hidden_size * 4);
+  l.blk = take((size_t)route_plan_blocks(r.n) * p->n_experts * 4);
+  l.mid = take((size_t)r.n * p->inter_size * 2);
+  l.part = take(r.owned ? 0 : (size_t)r.n * p->hidden_size * 4);
   l.total = at;
   return l;
 }
@@ -229,6 +262,8 @@ int check_moe(const exq_moe_problem* p) {
               (long long)p->n_experts, (long long)k);
   EXQ_REQUIRE(p->n_shared == 0 && p->group_size == 32,
               "%s: no shared experts, and groups of 32", fn);
+  EXQ_REQUIRE_SUPPORTED(T * H <= ((int64_t)1 << 30) - 1, "%s: T=%lld x H=%lld: hidden is past 2 GiB",
+                        fn, (long long)T, (long long)H);
   EXQ_REQUIRE_SUPPORTED(T <= ((int64_t)1 << 24) / k, "%s: T=%lld x k=%lld slots are too many", fn,
                         (long long)T, (long long)k);
   return EXQ_SUCCESS;
@@ -267,115 +302,83 @@ extern "C" int exq_moe_mxfp4_forward(const exq_moe_problem* p, const void* hidde
                      workspace_bytes, l.total);
   unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
   const hipStream_t s = as_stream(stream);
-  RoutePlanParams rp{};
-  rp.ids = topk_ids;
-  rp.ids_dtype = p->ids_dtype;
-  rp.T = (int)T;
-  rp.k = rp.kp = k;
-  rp.E = rp.Ep = E;
-  rp.n = (int)(T * k);
-  rp.all_tier = 2;
-  rp.hdr = reinterpret_cast<int*>(ws + l.hdr);
-  rp.ends = reinterpret_cast<int*>(ws + l.ends);
-  rp.sorted = reinterpret_cast<int*>(ws + l.sorted);
-  rp.tg = reinterpret_cast<TgEntry*>(ws + l.tg);
-  rp.tg_cap = (int)l.tg_cap;
-  const bool tile = T > (getenv("MXTH") ? atoi(getenv("MXTH")) : 64) && getenv("MXS") == nullptr;
-  rp.i4_group = rp.bf_group = rp.i8_group = rp.i4_big_group = tile ? kTileGroup : kGroup;
-  if (tile) rp.i4_big_rows = getenv("MXB") ? atoi(getenv("MXB")) : 33;
-  rp.out = out;
-  rp.out_bytes = T * H * 2;
-  rp.blk_cnt = reinterpret_cast<int*>(ws + l.blk);
-  const bool st_ = getenv("MXS") == nullptr && !tile;
-  const int64_t n = T * k;
-  const bool by_slot = st_ && T <= (getenv("MXT") ? atoi(getenv("MXT")) : 1) && n <= kOwnedSlots;
-  const bool all = st_ && !by_slot && T <= 16 && n <= 128 && E <= 256 && H <= 2048;
-  const bool route8 = st_ && !all && n <= 512 && E <= 512, route16 = st_ && !all && !route8 && n <= 1024 && E <= 256;
-  const bool route = by_slot || all || route8 || route16;
-  const bool owned = st_ && n <= kOwnedSlots;
-  if (!route) {
-    st = launch_route_plan(rp, s);
-    if (st) return st;
-  }
+  const Path r = path_of(p);
+  const bool bf = p->act_dtype == EXQ_DTYPE_BF16;
   MoeArgs a{};
-  a.hdr = rp.hdr;
-  a.tg = rp.tg;
-  a.sorted = rp.sorted;
+  a.hdr = reinterpret_cast<int*>(ws + l.hdr);
+  a.tg = reinterpret_cast<TgEntry*>(ws + l.tg);
+  a.sorted = reinterpret_cast<int*>(ws + l.sorted);
   a.top_k = k;
   a.mid = reinterpret_cast<uint16_t*>(ws + l.mid);
   a.part = reinterpret_cast<float*>(ws + l.part);
-  const bool bf = p->act_dtype == EXQ_DTYPE_BF16;
-  auto run = [&](bool gateup) {
-    a.x = gateup ? reinterpret_cast<const uint16_t*>(hidden) : a.mid;
-    a.tiles = reinterpret_cast<const uint4*>(gateup ? w13_tiles : w2_tiles);
-    a.wscales = reinterpret_cast<const uint32_t*>(gateup ? w13_scales : w2_scales);
-    a.K = (int)(gateup ? H : I);
-    a.N = (int)(gateup ? I : H);
-    a.KB = (int)tile_cols(a.K);
+  if (!r.by_slot && r.nseg == 0) {
+    RoutePlanParams rp{};
+    rp.ids = topk_ids;
+    rp.ids_dtype = p->ids_dtype;
+    rp.T = (int)T;
+    rp.k = rp.kp = k;
+    rp.E = rp.Ep = E;
+    rp.n = (int)r.n;
+    rp.all_tier = 2;
+    rp.hdr = a.hdr;
+    rp.ends = reinterpret_cast<int*>(ws + l.ends);
+    rp.sorted = a.sorted;
+    rp.tg = a.tg;
+    rp.tg_cap = (int)l.tg_cap;
+    rp.i4_group = rp.bf_group = rp.i8_group = rp.i4_big_group = kTileGroup;
+    rp.i4_big_rows = kTileGroup / 2 + 1;   // (the groups that take longest first)
+    rp.out = out;
+    rp.out_bytes = T * H * 2;
+    rp.blk_cnt = reinterpret_cast<int*>(ws + l.blk);
+    st = launch_route_plan(rp, s);
+    if (st) return st;
+  }
+  auto weights_of = [&](const uint8_t* tiles, const uint8_t* scales, int64_t K, int64_t N,
+                        int64_t rows, int gated) {
+    a.tiles = reinterpret_cast<const uint4*>(tiles);
+    a.wscales = reinterpret_cast<const uint32_t*>(scales);
+    a.K = (int)K;
+    a.N = (int)N;
+    a.KB = (int)tile_cols(K);
     a.G = (a.KB + 3) / 4;
-    a.RT = (int)(gateup ? mx::tile_rows(2 * I, 1) : mx::tile_rows(H, 0));
-    if (getenv("MXS") == nullptr && !tile) {
-      if (!gateup && owned) {
-        OwnedArgs o{by_slot ? nullptr : a.hdr, a.tg, a.sorted, a.mid, a.tiles, reinterpret_cast<const uint8_t*>(a.wscales), topk_ids, topk_weights,
-          p->ids_dtype, p->weights_dtype, (int)T, k, E, (int)I, (int)H, a.KB, a.G, a.RT, reinterpret_cast<uint16_t*>(out)};
-        if (bf) hipLaunchKernelGGL((moe_owned_down_kernel<true, 3>), dim3((unsigned)(H / 16)), dim3(512), 0, s, o);
-        else hipLaunchKernelGGL((moe_owned_down_kernel<false, 3>), dim3((unsigned)(H / 16)), dim3(512), 0, s, o);
-        return check_launch("moe_owned_down_kernel");
-      }
-      StreamArgs b{rp.hdr, rp.tg, rp.sorted, topk_ids, p->ids_dtype, (int)(T * k), E, a.x, a.tiles, reinterpret_cast<const uint8_t*>(a.wscales), a.K, a.KB, a.G, a.RT, a.top_k, a.N,
-                   0, 1, a.mid, a.part};
-      auto go = [&](auto kernel, int KS, int C) {
-        b.n_rt = (int)cdiv(a.RT / 2, 4 / KS);
-        b.chunks = (int)cdiv(cdiv(a.KB, KS), C);
-        const int64_t cap = tg_capacity(T * k, E, 16) * b.n_rt;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(cap < 512 ? cap : 512)), dim3(256), 0, s, b);
-        return check_launch("moe_stream_kernel");
-      };
-#define GO(UP, NSEG, ALL, KS, C) return bf ? go(moe_stream_kernel<true, UP, NSEG, ALL, KS, C>, KS, C) : go(moe_stream_kernel<false, UP, NSEG, ALL, KS, C>, KS, C)
-      if (gateup) {
-        if (by_slot) GO(true, kBySlot, false, 4, 4);
-        if (all) GO(true, 2, true, 4, 4);
-        if (route8) GO(true, 8, false, 4, 4);
-        if (route16) GO(true, 16, false, 4, 4);
-        GO(true, 0, false, 4, 4);
-      }
-      if (a.KB <= 6) GO(false, 0, false, 2, 3);
-      if (a.KB <= 8) GO(false, 0, false, 4, 2);
-      if (a.KB <= 12) GO(false, 0, false, 4, 3);
-      GO(false, 0, false, 4, 4);
-    }
-    if (tile) {
-      const int64_t cap = tg_capacity(T * k, E, kTileGroup);
-      const int rows = cap * cdiv(a.RT, 16) < (getenv("MXU") ? atoi(getenv("MXU")) : 512) ? 128 : 256;
-      auto go = [&](auto kernel) {
-        const int64_t nt = cdiv(a.RT, rows / 16);
-        hipLaunchKernelGGL(kernel, dim3((unsigned)spread_grid(cap, nt)), dim3(256), 0, s, a, (int)nt);
-        return check_launch("moe_tile_kernel");
-      };
-#define GT(UP) return rows == 128 ? bf ? go(moe_tile_kernel<true, UP, 2>) : go(moe_tile_kernel<false, UP, 2>) : bf ? go(moe_tile_kernel<true, UP, 4>) : go(moe_tile_kernel<false, UP, 4>)
-      if (gateup) GT(true);
-      GT(false);
-    }
-    const dim3 grid((unsigned)cdiv(cdiv(a.N, 16), 4), (unsigned)l.tg_cap);
-    if (gateup) {
-      if (bf) hipLaunchKernelGGL((moe_simple_kernel<true, true>), grid, dim3(256), 0, s, a);
-      else hipLaunchKernelGGL((moe_simple_kernel<false, true>), grid, dim3(256), 0, s, a);
-    } else {
-      if (bf) hipLaunchKernelGGL((moe_simple_kernel<true, false>), grid, dim3(256), 0, s, a);
-      else hipLaunchKernelGGL((moe_simple_kernel<false, false>), grid, dim3(256), 0, s, a);
-    }
-    return check_launch("moe_simple_kernel");
+    a.RT = (int)mx::tile_rows(rows, gated);
   };
-  st = run(true);
+  weights_of(w13_tiles, w13_scales, H, I, 2 * I, 1);
+  a.x = reinterpret_cast<const uint16_t*>(hidden);
+  if (r.by_slot) {
+    const SlotArgs b{topk_ids, p->ids_dtype, E, k, a.x, a.tiles,
+                     reinterpret_cast<const uint8_t*>(a.wscales), a.K, a.KB, a.G, a.RT, (int)I,
+                     a.mid};
+    const dim3 grid((unsigned)(I / 16), (unsigned)r.n);
+    if (bf) hipLaunchKernelGGL((moe_slot_gateup_kernel<true>), grid, dim3(256), 0, s, b);
+    else hipLaunchKernelGGL((moe_slot_gateup_kernel<false>), grid, dim3(256), 0, s, b);
+    st = check_launch("moe_slot_gateup_kernel");
+  } else {
+    const RouteArgs ra{topk_ids, p->ids_dtype, (int)r.n, E, k, a.hdr, a.tg, a.sorted};
+    st = bf ? launch_gateup<true>(a, ra, r, s) : launch_gateup<false>(a, ra, r, s);
+  }
   if (st) return st;
-  st = run(false);
-  if (st || owned) return st;
+  weights_of(w2_tiles, w2_scales, I, H, H, 0);
+  a.x = a.mid;
+  if (r.owned) {
+    const OwnedArgs o{r.by_slot ? nullptr : a.hdr, a.tg, a.sorted, a.mid, a.tiles,
+                      reinterpret_cast<const uint8_t*>(a.wscales), topk_ids, topk_weights,
+                      p->ids_dtype, p->weights_dtype, (int)T, k, E, (int)I, (int)H, a.KB, a.G,
+                      a.RT, reinterpret_cast<uint16_t*>(out)};
+    const dim3 grid((unsigned)(H / 16));
+    if (bf) hipLaunchKernelGGL((moe_owned_down_kernel<true, 3>), grid, dim3(64 * kOwnedWaves), 0, s, o);
+    else hipLaunchKernelGGL((moe_owned_down_kernel<false, 3>), grid, dim3(64 * kOwnedWaves), 0, s, o);
+    return check_launch("moe_owned_down_kernel");
+  }
+  st = bf ? launch_down<true>(a, l.tg_cap, s) : launch_down<false>(a, l.tg_cap, s);
+  if (st) return st;
   auto combine = [&](auto kernel, int cpl) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(T * (H / cpl), 256)), dim3(256), 0, s, a.part,
                        topk_ids, p->ids_dtype, topk_weights, p->weights_dtype, k, E, (int)H, (int)T,
                        reinterpret_cast<uint16_t*>(out));
     return check_launch("moe_combine_kernel");
   };
+  // two columns a lane until four fill the chip: 64 tokens x 2048 6.9 and 4.5 us
   if (T * H <= 256 * 512)
     return bf ? combine(moe_combine_kernel<true, 2>, 2) : combine(moe_combine_kernel<false, 2>, 2);
   return bf ? combine(moe_combine_kernel<true, 4>, 4) : combine(moe_combine_kernel<false, 4>, 4);

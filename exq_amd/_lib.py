@@ -106,6 +106,7 @@ _SIGNATURES = {
     "exq_dequantize_mxfp4": ([_P, _P, _I64, _I64, _P, _INT, _P], _INT),
     "exq_tile_mxfp4": ([_P, _P, _I64, _I64, _I64, _INT, _P, _P, _P], _INT),
     "exq_linear_mxfp4": ([C.POINTER(LinearProblem), _P, _P, _P, _P, _P, _P, _P, _P], _INT),
+    "exq_linear_mxfp4_kernel": ([C.POINTER(LinearProblem)], C.c_char_p),
     "exq_moe_mxfp4_workspace_size": ([C.POINTER(MoeProblem)], _SZ),
     "exq_moe_mxfp4_forward": ([C.POINTER(MoeProblem), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P], _INT),
     "exq_stream_read": ([_P, _I64, _P, _I64, _P], _INT),

@@ -8,7 +8,6 @@
 // ends with columns 4 q .. 4 q + 3 of a tile for token r.
 #include "mxfp4_tile.h"
 
-#include <stdlib.h>
 #include <type_traits>
 
 namespace exq {
@@ -24,62 +23,109 @@ struct MxArgs : LinArgs {   // x: 16-bit rows, or packed ones (ldx in bytes)
   int KB, G;                // tiles along the columns, groups of four of them
 };
 
-// One wave: 16 tokens x a tile of rows (gated: a gate and an up tile).
-template <bool BF, bool X4, bool GATED>
-__global__ void __launch_bounds__(256) mx_simple_kernel(MxArgs a, int nm, int nn) {
-  constexpr int NT = GATED ? 2 : 1;
-  const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t mb = unit / nn;
-  const int nb = (int)(unit - mb * nn);
-  if (mb >= nm) return;
-  const int64_t m = mb * 16 + r16 < a.T ? mb * 16 + r16 : a.T - 1;
-  const int K = (int)a.K, blocks = K / kBlock;
-  f32x4_t acc[NT] = {};
-  for (int kb = 0; kb < a.KB; ++kb) {
-    uint4 w[NT];
-    uint32_t s[NT];
+// ---- few tokens: a stream of weights --------------------------------------------------------
+// 16 MT tokens x a tile of weight rows (gated: a gate tile and its up tile) by W waves that
+// split the contraction; both operands straight from memory, and the sums joined through
+// LDS in wave order.
+template <bool BF, bool X4, bool GATED, int MT, int W>
+__global__ void __launch_bounds__(64 * W) mx_stream_kernel(MxArgs a, int nn) {
+  constexpr int NT = GATED ? 2 : 1, C = X4 || MT == 1 ? 4 : 2;   // tiles along K in flight
+  __shared__ __align__(16) float4 red[W * MT * NT * 64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, q = lane >> 4;
+  const int mb = blockIdx.x / nn, nb = blockIdx.x - mb * nn;
+  const int64_t m0 = (int64_t)mb * MT * 16;
+  const int blocks = (int)(a.K / kBlock);
+  const uint8_t* w8 = reinterpret_cast<const uint8_t*>(a.wscales);
+  const uint8_t *x[MT], *xs[MT];   // (rows past the last repeat it: what they give is not stored)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int64_t rt = (int64_t)nb * NT + t;
-      w[t] = a.tiles[(rt * a.KB + kb) * 64 + lane];
-      s[t] = a.wscales[(rt * a.G + (kb >> 2)) * 64 + lane] >> (8 * (kb & 3)) & 0xff;
-    }
-    const int b = kb * 4 + q;
-    if constexpr (X4) {
-      uint4 x = uint4{0u, 0u, 0u, 0u};
-      int sx = 0;
-      if (b < blocks) {
-        x = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.x) + m * a.ldx +
-                                            b * 16);
-        sx = a.xs[m * blocks + b];
-      }
+  for (int u = 0; u < MT; ++u) {
+    const int64_t m = m0 + u * 16 + r16 < a.T ? m0 + u * 16 + r16 : a.T - 1;
+    x[u] = reinterpret_cast<const uint8_t*>(a.x) + m * a.ldx * (X4 ? 1 : 2);
+    xs[u] = X4 ? a.xs + m * blocks : nullptr;
+  }
+  const int kb0 = wave * a.KB / W, kb1 = (wave + 1) * a.KB / W;
+  f32x4_t acc[MT][NT] = {};
+  for (int k0 = kb0; k0 < kb1; k0 += C) {
+    uint4 w[C][NT], v[C][MT][X4 ? 1 : 4];
+    uint32_t s[C][NT], sx[C][MT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t] = mfma_mx(w[t], (int)s[t], x, sx, acc[t]);
-    } else {
-      uint4 x[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        x[j] = b < blocks ? *reinterpret_cast<const uint4*>(a.x + m * a.ldx + b * 32 + j * 8)
-                          : uint4{0u, 0u, 0u, 0u};
+    for (int c = 0; c < C; ++c) {
+      const int kb = k0 + c < kb1 ? k0 + c : kb1 - 1;   // (past the range: loaded again, not used)
+      const int b = kb * 4 + q < blocks ? kb * 4 + q : blocks - 1;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const uint32_t c[4] = {w[t].x, w[t].y, w[t].z, w[t].w};
+        const int64_t rt = (int64_t)nb * NT + t;
+        w[c][t] = a.tiles[(rt * a.KB + kb) * 64 + lane];
+        s[c][t] = w8[((rt * a.G + (kb >> 2)) * 64 + lane) * 4 + (kb & 3)];
+      }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[t] = dev::dmfma<BF>(decode8<BF>(c[j], __uint_as_float(s[t] << 23)), x[j], acc[t]);
+      for (int u = 0; u < MT; ++u) {
+        if constexpr (X4) {
+          v[c][u][0] = *reinterpret_cast<const uint4*>(x[u] + b * 16);
+          sx[c][u] = xs[u][b];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            v[c][u][j] = *reinterpret_cast<const uint4*>(x[u] + b * 64 + j * 16);
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (k0 + c >= kb1) break;
+      const bool in = (k0 + c) * 4 + q < blocks;        // (columns past K: zeros)
+#pragma unroll
+      for (int u = 0; u < MT; ++u)
+#pragma unroll
+        for (int j = 0; j < (X4 ? 1 : 4); ++j)
+          if (!in) v[c][u][j] = uint4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (X4) {
+#pragma unroll
+          for (int u = 0; u < MT; ++u)
+            acc[u][t] = mfma_mx(w[c][t], (int)s[c][t], v[c][u][0], in ? (int)sx[c][u] : 0,
+                                acc[u][t]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 d = decode8<BF>(j == 0   ? w[c][t].x
+                                        : j == 1 ? w[c][t].y
+                                        : j == 2 ? w[c][t].z
+                                                 : w[c][t].w,
+                                        __uint_as_float(s[c][t] << 23));
+#pragma unroll
+            for (int u = 0; u < MT; ++u) acc[u][t] = dev::dmfma<BF>(d, v[c][u][j], acc[u][t]);
+          }
+        }
       }
     }
   }
-  const int64_t mo = mb * 16 + r16, n = (int64_t)nb * 16 + q * 4;
-  float y[4], u[4], res[4];
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    y[v] = acc[0][v];
-    u[v] = acc[NT - 1][v];
+  for (int u = 0; u < MT; ++u)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      red[((wave * MT + u) * NT + t) * 64 + lane] =
+          float4{acc[u][t][0], acc[u][t][1], acc[u][t][2], acc[u][t][3]};
+  __syncthreads();
+  for (int u = wave; u < MT; u += W) {
+    const int64_t m = m0 + u * 16 + r16, n = (int64_t)nb * 16 + q * 4;
+    float y[4], up[4], res[4];
+    if constexpr (!GATED) fetch_residual<4>(a, m, n, res);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float4 sum = red[(u * NT + t) * 64 + lane];
+#pragma unroll
+      for (int k = 1; k < W; ++k) {
+        const float4 p = red[((k * MT + u) * NT + t) * 64 + lane];
+        sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+      }
+      float* o = t ? up : y;
+      o[0] = sum.x; o[1] = sum.y; o[2] = sum.z; o[3] = sum.w;
+    }
+    finish_run<4, GATED>(a, m, n, y, up, res);
   }
-  if constexpr (!GATED) fetch_residual<4>(a, mo, n, res);
-  finish_run<4, GATED>(a, mo, n, y, u, res);
 }
 
 // ---- many tokens: tiles -------------------------------------------------------------------
@@ -144,23 +190,77 @@ int launch_tile(const MxArgs& a, hipStream_t s) {
   return check_launch("mx_tile_kernel");
 }
 
-template <bool BF, bool X4, bool GATED>
-int launch_products(const MxArgs& a, hipStream_t s) {
-  const char* v = getenv("MXV");
-  if constexpr (X4) if (v && v[0] == '0') return launch_tile<BF, X4, GATED, 2, 2, 8, 8, 2>(a, s);
-  if (v && v[0] == '1') return launch_tile<BF, X4, GATED, 1, 4, 8, 4, 2>(a, s);
-  if (v && v[0] == '2') return launch_tile<BF, X4, GATED, 1, 4, 4, 4, 3>(a, s);
-  if (v && v[0] == '3') return launch_tile<BF, X4, GATED, 1, 4, 4, 2, 3>(a, s);
-  if (v && v[0] == '4') return launch_tile<BF, X4, GATED, 1, 4, 2, 2, 6>(a, s);
-  if (v && v[0] == '5') return launch_tile<BF, X4, GATED, 1, 4, 2, 4, 5>(a, s);
-  if (v && v[0] == '6') return launch_tile<BF, X4, GATED, 1, 4, 4, 4, 2>(a, s);
-  const int64_t nm = cdiv(a.T, 16), nn = cdiv(a.N, 16), grid = cdiv(nm * nn, 4);
-  EXQ_REQUIRE_SUPPORTED(grid * 256 < ((int64_t)1 << 32),
+template <bool BF, bool X4, bool GATED, int MT, int W>
+int launch_stream(const MxArgs& a, hipStream_t s) {
+  const int64_t nm = cdiv(a.T, 16 * MT), nn = cdiv(a.N, 16), grid = nm * nn;
+  EXQ_REQUIRE_SUPPORTED(grid * 64 * W < ((int64_t)1 << 32),
                         "exq_linear_mxfp4: T=%lld x N=%lld is too large", (long long)a.T,
                         (long long)a.N);
-  hipLaunchKernelGGL((mx_simple_kernel<BF, X4, GATED>), dim3((unsigned)grid), dim3(256), 0, s, a,
-                     (int)nm, (int)nn);
-  return check_launch("mx_simple_kernel");
+  hipLaunchKernelGGL((mx_stream_kernel<BF, X4, GATED, MT, W>), dim3((unsigned)grid), dim3(64 * W),
+                     0, s, a, (int)nn);
+  return check_launch("mx_stream_kernel");
+}
+
+// Which kernel: the one with the least rounds x time of a round.  ns[i]: what 128 columns of
+// K take when every CU holds i + 1 of the work-groups (three is a round), measured in bf16
+// and in MXFP4 tokens with K = 4096; it does not move with K.  In us for 16, 32, 64, 128, 512
+// and 2048 tokens x 4096 x 4096:
+//   bf16    16 x 16 stream 7.7, 12.1, 20, -, -, -      32 x 16 stream 8.7, 11.3, 19, 34, -, -
+//           32 x 128 tiles 16, 17, 17, 17.7, 24.5, 79  32 x 256 23, 25, 25, 25, 26.6, 70
+//           64 x 256 33, 35, 39, 39, 41, 65
+//   MXFP4   16 x 16 6.0, 8.4, 12.9, -, -, -   32 x 16 6.3, 7.8, 12, 20, 37 (256), -
+//           32 x 128 17, 21, 21, 21, 25, 84   32 x 256 21, 26, 26, 26, 27, 61
+//           64 x 256 23, 28, 38, 37, 38, 58   256 x 256 -, -, -, -, 95, 96
+// and 4096 tokens x 14336 x 4096: 64 x 256 bf16 351, MXFP4 311 and 256 x 256 249.
+// A gated stream's work-group makes a gate and an up tile in the time of one (16 tokens x 2048
+// x 2816 5.5 us: the tokens take it); up to four tokens cost less, as their rows are few.
+struct Shape {
+  int tokens, rows;
+  int ns[3], ns4[3];
+};
+constexpr int kFewTokens = 4;
+constexpr Shape kFew = {16, 16, {80, 150, 210}, {66, 120, 170}};
+constexpr Shape kShapes[] = {
+    {16, 16, {147, 280, 410}, {94, 170, 240}},       // streams
+    {32, 16, {260, 500, 730}, {150, 280, 400}},
+    {32, 128, {450, 670, 930}, {580, 690, 990}},     // tiles
+    {32, 256, {740, 1140, 1590}, {750, 920, 1300}},
+    {64, 256, {1280, 1950, 2420}, {1140, 1710, 2080}},
+    {256, 256, {0, 0, 0}, {2220, 4440, 6660}},
+};
+constexpr const char* kKernels[] = {"stream 16x16", "stream 32x16", "tile 32x128",
+                                    "tile 32x256",  "tile 64x256",  "tile 256x256"};
+
+int pick_kernel(int64_t tokens, int64_t rows, bool x4, bool gated) {
+  int best = 0;
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < (int)(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {
+    const Shape& k = i == 0 && tokens <= kFewTokens ? kFew : kShapes[i];
+    const int* ns = x4 ? k.ns4 : k.ns;
+    if (ns[0] == 0) continue;
+    const int64_t rows_of = gated && k.rows == 16 ? 32 : k.rows;
+    const int64_t per_cu = cdiv(cdiv(tokens, k.tokens) * cdiv(rows, rows_of), 256);
+    const int64_t rest = per_cu % 3, t = per_cu / 3 * ns[2] + (rest ? ns[rest - 1] : 0);
+    if (t < least) {
+      least = t;
+      best = i;
+    }
+  }
+  return best;
+}
+
+template <bool BF, bool X4, bool GATED>
+int launch_products(const MxArgs& a, hipStream_t s) {
+  switch (pick_kernel(a.T, a.N * (GATED ? 2 : 1), X4, GATED)) {
+    case 0: return launch_stream<BF, X4, GATED, 1, 8>(a, s);
+    case 1: return launch_stream<BF, X4, GATED, 2, 8>(a, s);
+    case 2: return launch_tile<BF, X4, GATED, 1, 4, 2, 2, 6>(a, s);
+    case 3: return launch_tile<BF, X4, GATED, 1, 4, 2, 4, 5>(a, s);
+    case 4: return launch_tile<BF, X4, GATED, 1, 4, 4, 4, 3>(a, s);
+    default:
+      if constexpr (X4) return launch_tile<BF, X4, GATED, 2, 2, 8, 8, 2>(a, s);
+      return EXQ_ERROR_UNSUPPORTED;  // (not reached: 16-bit tokens have no such shape)
+  }
 }
 
 }  // namespace
@@ -168,14 +268,12 @@ int launch_products(const MxArgs& a, hipStream_t s) {
 
 using namespace exq;
 
-extern "C" int exq_linear_mxfp4(const exq_linear_problem* p, const void* x,
-                                const uint8_t* x_scales, const uint8_t* tiles,
-                                const uint8_t* tile_scales, const void* bias,
-                                const void* residual, void* out, exq_stream stream) {
+namespace {
+int check_problem(const exq_linear_problem* p, const void* bias, const void* residual) {
   const char* fn = "exq_linear_mxfp4";
   EXQ_REQUIRE(p, "%s: null problem", fn);
-  const bool x4 = p->act_dtype == EXQ_DTYPE_U8;
-  EXQ_REQUIRE(x4 || is_act_dtype(p->act_dtype), "%s: x must be f16, bf16 or u8 (MXFP4)", fn);
+  EXQ_REQUIRE(p->act_dtype == EXQ_DTYPE_U8 || is_act_dtype(p->act_dtype),
+              "%s: x must be f16, bf16 or u8 (MXFP4)", fn);
   EXQ_REQUIRE(is_float_dtype(p->out_dtype), "%s: out dtype must be f32, f16 or bf16", fn);
   EXQ_REQUIRE(!bias || is_float_dtype(p->bias_dtype), "%s: bias dtype must be f32, f16 or bf16",
               fn);
@@ -185,12 +283,28 @@ extern "C" int exq_linear_mxfp4(const exq_linear_problem* p, const void* x,
               "%s: unknown activation %d", fn, p->activation);
   EXQ_REQUIRE(!(p->gated && residual), "%s: a gated product takes no residual", fn);
   const int64_t T = p->n_tokens, K = p->in_features, N = p->out_features;
-  EXQ_REQUIRE(T >= 0 && T <= INT32_MAX / 2 && K >= mx::kBlock && K <= (1 << 24) &&
+  EXQ_REQUIRE(T >= 0 && T <= INT32_MAX / 2 && K >= mx::kBlock && K <= (1 << 22) &&
                   K % mx::kBlock == 0 && N >= 1 && N <= (1 << 20),
               "%s: sizes T=%lld K=%lld N=%lld out of range (K a multiple of 32)", fn,
               (long long)T, (long long)K, (long long)N);
   EXQ_REQUIRE(p->x_stride >= 0 && p->residual_stride >= 0 && (T <= 1 || p->out_stride >= N),
               "%s: row strides must not be negative, and out's at least N", fn);
+  // (a tile's rows of x lie in one buffer resource)
+  EXQ_REQUIRE_SUPPORTED(T <= 1 || p->x_stride <= (1 << 22), "%s: x's row stride %lld is too large",
+                        fn, (long long)p->x_stride);
+  return EXQ_SUCCESS;
+}
+}  // namespace
+
+extern "C" int exq_linear_mxfp4(const exq_linear_problem* p, const void* x,
+                                const uint8_t* x_scales, const uint8_t* tiles,
+                                const uint8_t* tile_scales, const void* bias,
+                                const void* residual, void* out, exq_stream stream) {
+  const char* fn = "exq_linear_mxfp4";
+  const int status = check_problem(p, bias, residual);
+  if (status != EXQ_SUCCESS) return status;
+  const bool x4 = p->act_dtype == EXQ_DTYPE_U8;
+  const int64_t T = p->n_tokens, K = p->in_features, N = p->out_features;
   if (T == 0) return EXQ_SUCCESS;
   EXQ_REQUIRE(x && tiles && tile_scales && out && (!x4 || x_scales), "%s: null pointer", fn);
   EXQ_REQUIRE(((uintptr_t)x | (uintptr_t)tiles | (uintptr_t)tile_scales) % 16 == 0 &&
@@ -228,4 +342,10 @@ extern "C" int exq_linear_mxfp4(const exq_linear_problem* p, const void* x,
                     : launch_products<true, false, false>(a, s);
   return p->gated ? launch_products<false, false, true>(a, s)
                   : launch_products<false, false, false>(a, s);
+}
+
+extern "C" const char* exq_linear_mxfp4_kernel(const exq_linear_problem* p) {
+  if (check_problem(p, nullptr, nullptr) != EXQ_SUCCESS || p->n_tokens == 0) return nullptr;
+  return kKernels[pick_kernel(p->n_tokens, p->out_features * (p->gated ? 2 : 1),
+                              p->act_dtype == EXQ_DTYPE_U8, p->gated != 0)];
 }

@@ -254,7 +254,8 @@ def _call(x, weight, bias, x_scales, activation, residual, out_dtype, out, gated
     _refuse_gradients(what, x, bias, residual, out)
     dev = _device(x, tiles, tile_scales, bias, x_scales, residual, out)
     _check_start(tiles, tile_scales)
-    if x.data_ptr() % 16 or (p.n_tokens > 1 and p.x_stride * x.element_size() % 16):
+    if x.data_ptr() % 16 or (p.n_tokens > 1 and (p.x_stride * x.element_size() % 16
+                                                 or p.x_stride > 1 << 22)):
         x = x.clone(memory_format=torch.contiguous_format)   # (rows at 16-byte addresses)
         p = _problem(_layout(x), *layouts)
     if out is None:
@@ -285,7 +286,8 @@ def fused_linear_mxfp4(x: torch.Tensor, weight: Mxfp4Weight, bias: torch.Tensor 
     operands go to the 4-bit matrix instructions.  bias, residual, ``activation`` and
     ``out`` as in ``fused_linear``; returns [T, N] in ``out_dtype`` (default x's,
     bfloat16 for packed x).  Sums in float32, one rounding at the end.  x's row stride
-    is free; rows that do not start at 16-byte addresses are copied first.
+    is free; rows that do not start at 16-byte addresses, or lie more than 2^22
+    elements apart, are copied first.
     Stream-ordered, graph-capturable, no workspace, no derivative (as ``fused_linear``).
     """
     if activation not in _ACTIVATIONS:

@@ -360,8 +360,8 @@ int exq_tile_mxfp4(const uint8_t* packed, const uint8_t* scales, int64_t n_matri
  * x [T, K] is 16-bit and the weight's values take its type, exact in bf16, rounded to
  * nearest in f16 (exact for scales 2^-23 .. 2^13); x_scales is not read.  act_dtype u8: x
  * [T, K/2] is MXFP4 too, x_stride bytes from row to row, with x_scales [T, K/32].
- * Products are summed in fp32 and the result is rounded once, to out_dtype.  x's rows,
- * tiles and tile_scales are 16-byte aligned.  out may be residual itself (same pointer,
+ * Products are summed in fp32 and the result is rounded once, to out_dtype.  x's rows
+ * (at most 2^22 elements apart), tiles and tile_scales are 16-byte aligned; K <= 2^22.  out may be residual itself (same pointer,
  * dtype and stride) and must not overlap any other input.  No workspace.
  */
 int exq_linear_mxfp4(const exq_linear_problem* problem, const void* x, const uint8_t* x_scales,
@@ -576,6 +576,9 @@ int exq_stream_read(const void* buf, int64_t bytes, uint32_t* sink, int64_t sink
  */
 const char* exq_linear_kernel(const exq_linear_problem* problem, const void* x,
                               const void* weight);
+
+/* The same for exq_linear_mxfp4 (the choice depends on the problem alone). */
+const char* exq_linear_mxfp4_kernel(const exq_linear_problem* problem);
 
 #ifdef __cplusplus
 }

@@ -14,6 +14,7 @@ import torch
 
 from oracle import dense, mxfp4
 from tests._helpers import banner
+from tests._mxfp4_cases import cases
 
 pytestmark = pytest.mark.gpu
 
@@ -189,6 +190,37 @@ def test_whole_numbers(T, K, N, kind, gated, device):
     out = fused_linear_mxfp4(x, w, b.to(o).cuda(), x_scales=x_scales, residual=r.to(o).cuda(), out_dtype=o)
     want = (y + b + r).float().to(o)
     assert torch.equal(out.cpu(), want), _where(out.cpu(), want)
+
+
+@pytest.mark.parametrize("x4,gated,kernel,T,N", cases())
+@pytest.mark.parametrize("K", [96, 672])
+def test_every_kernel_at_its_edges(x4, gated, kernel, T, N, K, device):
+    """Whole numbers, the sums computed on the GPU in 64 bits from the oracle's values."""
+    from exq_amd.kernels import Mxfp4Weight, fused_gated_linear_mxfp4, fused_linear_mxfp4
+    banner(f"mxfp4 {kernel} x4={x4} gated={gated} T={T} N={N} K={K}")
+    rows = 2 * N if gated else N
+    packed, scales = _codes(rows, K, 1, 0, 0)
+    if gated:       # (as above: the product of two sums has to be exact)
+        keep = torch.zeros(K // 2, dtype=torch.uint8)
+        keep[torch.randperm(K // 2, generator=torch.Generator().manual_seed(9))[:8]] = 255
+        packed &= keep
+    w = Mxfp4Weight.from_packed(packed.cuda(), scales.cuda(), gated)
+    if x4:
+        xp, xs = _codes(T, K, 2, -1, -1)
+        x, x_scales, X = xp.cuda(), xs.cuda(), _dense(xp, xs).cuda()
+    else:
+        X = torch.randint(-3, 4, (T, K), generator=torch.Generator().manual_seed(2)).double().cuda()
+        x, x_scales = X.to(torch.bfloat16), None
+    y = torch.mm(X, _dense(packed, scales).cuda().t())
+    hold = torch.full((T + 1, N + 3), 7.0, device="cuda")
+    if gated:
+        fused_gated_linear_mxfp4(x, w, x_scales=x_scales, activation="relu", out=hold[:T, :N])
+        want = (torch.relu(y[:, :N]) * y[:, N:]).float()
+    else:
+        fused_linear_mxfp4(x, w, x_scales=x_scales, out=hold[:T, :N])
+        want = y.float()
+    assert torch.equal(hold[:T, :N], want), _where(hold[:T, :N], want)
+    assert (hold[T] == 7.0).all() and (hold[:, N:] == 7.0).all()
 
 
 def _bounded(X, W, bias, act, residual, out, gated):

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(64 * W) mx_stream_kernel(MxArgs a, int nn) {
 
 // ---- many tokens: tiles -------------------------------------------------------------------
 template <bool BF, bool X4, bool GATED, int WM, int WN, int MT, int NT, int P>
-__global__ void __launch_bounds__(64 * WM * WN, MT == 8 ? 1 : X4 ? 2 : 3) mx_tile_kernel(MxArgs a, int nm, int nn) {
+__global__ void __launch_bounds__(64 * WM * WN, X4 && MT == 8 ? 2 : 3) mx_tile_kernel(MxArgs a, int nm, int nn) {
   using T = std::conditional_t<X4, Tile4<WM, WN, MT, NT>, Tile16<BF, WM, WN, MT, NT, P>>;
   constexpr int COLS = (GATED ? 8 : 16) * NT;      // output columns of a wave
   constexpr int SUMS = T::W * wave_floats<NT>() * 4;
@@ -157,12 +157,8 @@ __global__ void __launch_bounds__(64 * WM * WN, MT == 8 ? 1 : X4 ? 2 : 3) mx_til
   f32x4_t acc[MT][NT] = {};
   if constexpr (X4) {
     const uint8_t* x = reinterpret_cast<const uint8_t*>(a.x);
-    const uint8_t* xs[MT];
-#pragma unroll
-    for (int u = 0; u < MT; ++u) {
-      const int64_t m = m0 + (wm * MT + u) * 16 + (lane & 15);
-      xs[u] = a.xs + (m < a.T ? m : a.T - 1) * blocks;
-    }
+    const int64_t m = m0 + threadIdx.x;
+    const uint8_t* xs = a.xs + (m < a.T ? m : a.T - 1) * blocks;
     T::run(lds, uniform_rsrc(x + m0 * a.ldx), vo, xs, a.tiles,
            a.wscales, rt, a.KB, a.G, blocks, wave, lane, acc);
   } else {
@@ -209,9 +205,11 @@ int launch_stream(const MxArgs& a, hipStream_t s) {
 //           32 x 128 tiles 16, 17, 17, 17.7, 24.5, 79  32 x 256 23, 25, 25, 25, 26.6, 70
 //           64 x 256 33, 35, 39, 39, 41, 65
 //   MXFP4   16 x 16 6.0, 8.4, 12.9, -, -, -   32 x 16 6.3, 7.8, 12, 20, 37 (256), -
-//           32 x 128 17, 21, 21, 21, 25, 84   32 x 256 21, 26, 26, 26, 27, 61
-//           64 x 256 23, 28, 38, 37, 38, 58   256 x 256 -, -, -, -, 95, 96
-// and 4096 tokens x 14336 x 4096: 64 x 256 bf16 351, MXFP4 311 and 256 x 256 249.
+//           32 x 128 -, -, 13, 13.5, 15.5, 41  32 x 256 -, -, 17, 17, 18, 40
+//           64 x 256 -, -, 23, 23, 24, 33      128 x 256 -, -, 29, 36, 37, 40
+//           256 x 256 -, -, 37, 45, 45, 48
+// and 4096 tokens x 14336 x 4096: bf16 64 x 256 351; MXFP4 64 x 256 190, 128 x 256 153, 256 x
+// 256 (eight waves) 143; gated 4096 x 4096 x 14336: bf16 64 x 256 711, MXFP4 333, 294 and 301.
 // A gated stream's work-group makes a gate and an up tile in the time of one (16 tokens x 2048
 // x 2816 5.5 us: the tokens take it); up to four tokens cost less, as their rows are few.
 struct Shape {
@@ -223,13 +221,14 @@ constexpr Shape kFew = {16, 16, {80, 150, 210}, {66, 120, 170}};
 constexpr Shape kShapes[] = {
     {16, 16, {147, 280, 410}, {94, 170, 240}},       // streams
     {32, 16, {260, 500, 730}, {150, 280, 400}},
-    {32, 128, {450, 670, 930}, {580, 690, 990}},     // tiles
-    {32, 256, {740, 1140, 1590}, {750, 920, 1300}},
-    {64, 256, {1280, 1950, 2420}, {1140, 1710, 2080}},
-    {256, 256, {0, 0, 0}, {2220, 4440, 6660}},
+    {32, 128, {450, 670, 930}, {330, 390, 470}},     // tiles
+    {32, 256, {740, 1140, 1590}, {480, 670, 850}},
+    {64, 256, {1280, 1950, 2420}, {680, 950, 1250}},
+    {128, 256, {0, 0, 0}, {1140, 1500, 2000}},
+    {256, 256, {0, 0, 0}, {1400, 2720, 4080}},
 };
-constexpr const char* kKernels[] = {"stream 16x16", "stream 32x16", "tile 32x128",
-                                    "tile 32x256",  "tile 64x256",  "tile 256x256"};
+constexpr const char* kKernels[] = {"stream 16x16", "stream 32x16", "tile 32x128", "tile 32x256",
+                                    "tile 64x256",  "tile 128x256", "tile 256x256"};
 
 int pick_kernel(int64_t tokens, int64_t rows, bool x4, bool gated) {
   int best = 0;
@@ -251,14 +250,18 @@ int pick_kernel(int64_t tokens, int64_t rows, bool x4, bool gated) {
 
 template <bool BF, bool X4, bool GATED>
 int launch_products(const MxArgs& a, hipStream_t s) {
-  switch (pick_kernel(a.T, a.N * (GATED ? 2 : 1), X4, GATED)) {
+  const int kernel = pick_kernel(a.T, a.N * (GATED ? 2 : 1), X4, GATED);
+  switch (kernel) {
     case 0: return launch_stream<BF, X4, GATED, 1, 8>(a, s);
     case 1: return launch_stream<BF, X4, GATED, 2, 8>(a, s);
     case 2: return launch_tile<BF, X4, GATED, 1, 4, 2, 2, 6>(a, s);
     case 3: return launch_tile<BF, X4, GATED, 1, 4, 2, 4, 5>(a, s);
     case 4: return launch_tile<BF, X4, GATED, 1, 4, 4, 4, 3>(a, s);
     default:
-      if constexpr (X4) return launch_tile<BF, X4, GATED, 2, 2, 8, 8, 2>(a, s);
+      if constexpr (X4) {
+        if (kernel == 5) return launch_tile<BF, X4, GATED, 1, 4, 8, 4, 2>(a, s);
+        return launch_tile<BF, X4, GATED, 2, 4, 8, 4, 2>(a, s);
+      }
       return EXQ_ERROR_UNSUPPORTED;  // (not reached: 16-bit tokens have no such shape)
   }
 }

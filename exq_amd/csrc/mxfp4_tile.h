@@ -159,94 +159,110 @@ struct Tile16 {
 };
 
 // The same with tokens in MXFP4: a stage is 256 columns, 128 bytes a row, eight pieces,
-// piece c of row r at place c ^ swz(r); both operands go to the matrix instructions as
-// they are, the tokens' scale bytes from memory.  A copy is eight rows.
+// piece c of row r at place c ^ swz8(r); a copy is eight rows.  Both operands go to the
+// matrix instructions as they are.  A token's eight scale bytes of a stage are one load of
+// one lane, a stage ahead, and lie behind the rows in LDS: straight from memory they were
+// 2 MT one-byte loads of every wave, 16 lines each, which took longer than the products.
 __device__ __forceinline__ int swz8(int r) { return (r >> 1) & 7; }
+struct __attribute__((packed, aligned(1))) Bytes8 {
+  uint32_t d[2];
+};
 
 template <int WM, int WN, int MT, int NT>
 struct Tile4 {
   static constexpr int W = WM * WN;
   static constexpr int BM = 16 * MT * WM, BR = 16 * NT * WN;
-  static constexpr int STAGE = BM * 128;
+  static constexpr int ROWS = BM * 128, STAGE = ROWS + BM * 8;
   static constexpr int D = BM / 8 / W;
   static constexpr int LDS = 2 * STAGE;
-  static_assert(BM % (8 * W) == 0 && W % 2 == 0 && LDS <= 160 * 1024, "copies");
+  static_assert(BM % (8 * W) == 0 && W % 2 == 0 && BM <= 64 * W && LDS <= 160 * 1024, "copies");
 
-  __device__ __forceinline__ static int row(int wave, int lane, int j) { return (j * W + wave) * 8 + (lane >> 3); }
+  __device__ __forceinline__ static int row(int wave, int lane, int j) {
+    return (j * W + wave) * 8 + (lane >> 3);
+  }
   __device__ __forceinline__ static int piece(int wave, int lane) {
     return (lane & 7) ^ swz8((wave * 8 + (lane >> 3)) & 15);
   }
 
-  // xs[u]: the scale bytes of the wave's token r16 of tile u, `blocks` of them.
-  __device__ __forceinline__ static void run(unsigned char* lds, __amdgpu_buffer_rsrc_t xr, const int (&vo)[D],
-                             const uint8_t* const (&xs)[MT], const uint4* tiles,
-                             const uint32_t* scales, const int (&rt)[NT], int KB, int G,
-                             int blocks, int wave, int lane, f32x4_t (&acc)[MT][NT]) {
-    const int r16 = lane & 15, q = lane >> 4, wm = wave / WN;
+  // xs: the scale bytes of token 64 wave + lane of the work-group, `blocks` of them.
+  __device__ __forceinline__ static void run(unsigned char* lds, __amdgpu_buffer_rsrc_t xr,
+                                             const int (&vo)[D], const uint8_t* xs,
+                                             const uint4* tiles, const uint32_t* scales,
+                                             const int (&rt)[NT], int KB, int G, int blocks,
+                                             int wave, int lane, f32x4_t (&acc)[MT][NT]) {
+    const int r16 = lane & 15, q = lane >> 4, wm = wave / WN, tid = wave * 64 + lane;
     const int pc = piece(wave, lane);
     const uint32_t lds0 = lds_offset(lds) + wave * 1024;
+    uint4 w[2][NT];
+    uint32_t s[2][NT];
+    uint2 b = uint2{0u, 0u};
+    // the tokens of stage kk and their scales
     auto copy = [&](int kk) {
       const uint32_t at = lds0 + (kk & 1) * STAGE;
       const bool in = kk * 8 + pc < blocks;
 #pragma unroll
       for (int j = 0; j < D; ++j) dma16(xr, at + j * W * 1024, in ? vo[j] : kOob, kk * 128);
-    };
-    uint4 w[2][NT];
-    uint32_t s[NT], b[2][MT];
-    auto load = [&](int kk) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int kb = 2 * kk + h < KB ? 2 * kk + h : KB - 1;   // (columns past K: x is zero)
-        const int bl = kb * 4 + q < blocks ? kb * 4 + q : blocks - 1;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) w[h][t] = tiles[((int64_t)rt[t] * KB + kb) * 64 + lane];
-#pragma unroll
-        for (int u = 0; u < MT; ++u) b[h][u] = xs[u][bl];
+      if (tid < BM) {
+        if (kk * 8 + 8 <= blocks) {
+          const Bytes8 v = *reinterpret_cast<const Bytes8*>(xs + kk * 8);
+          b = uint2{v.d[0], v.d[1]};
+        } else {
+          b = uint2{0u, 0u};
+          for (int i = 0; kk * 8 + i < blocks; ++i) {
+            const uint32_t v = (uint32_t)xs[kk * 8 + i] << (8 * (i & 3));
+            if (i < 4) b.x |= v; else b.y |= v;
+          }
+        }
       }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) s[t] = scales[((int64_t)rt[t] * G + (kk >> 1)) * 64 + lane];
     };
-    copy(0);
-    load(0);
-    const int rd = (wm * MT * 16 + r16) * 128, fr = swz8(r16);
-    const int KK = (KB + 1) >> 1;
-    for (int kk = 0; kk < KK; ++kk) {
-      wait_vm<0>();
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      uint4 wc[2][NT];
-      uint32_t sc[NT], bc[2][MT];
+    // the weights of its half h (columns past K: x is zero)
+    auto load = [&](int kk, int h) {
+      const int kb = 2 * kk + h < KB ? 2 * kk + h : KB - 1;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        wc[0][t] = w[0][t];
-        wc[1][t] = w[1][t];
-        sc[t] = s[t] >> (16 * (kk & 1));
+        w[h][t] = tiles[((int64_t)rt[t] * KB + kb) * 64 + lane];
+        s[h][t] = scales[((int64_t)rt[t] * G + (kb >> 2)) * 64 + lane];
       }
-#pragma unroll
-      for (int u = 0; u < MT; ++u) {
-        bc[0][u] = b[0][u];
-        bc[1][u] = b[1][u];
-      }
-      if (kk + 1 < KK) {
-        copy(kk + 1);
-        load(kk + 1);
-      }
-      const unsigned char* at = lds + (kk & 1) * STAGE + rd;
+    };
+    copy(0);
+    load(0, 0);
+    load(0, 1);
+    const int m0 = wm * MT * 16 + r16, fr = swz8(r16);
+    const int KK = (KB + 1) >> 1;
+    for (int kk = 0; kk < KK; ++kk) {
+      unsigned char* stage = lds + (kk & 1) * STAGE;
+      wait_vm<4 * NT>();   // all but the weights, whose registers the compiler waits for
+      if (tid < BM) *reinterpret_cast<uint2*>(stage + ROWS + tid * 8) = b;
+      wait_lds();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (kk + 1 < KK) copy(kk + 1);
+      const unsigned char* at = stage + m0 * 128;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint4 x[MT];
+        int sx[MT];
 #pragma unroll
-        for (int u = 0; u < MT; ++u)
+        for (int u = 0; u < MT; ++u) {
           x[u] = *reinterpret_cast<const uint4*>(at + u * 2048 + (((4 * h + q) ^ fr) * 16));
+          sx[u] = stage[ROWS + (m0 + u * 16) * 8 + h * 4 + q];
+        }
+        const int shift = 8 * ((2 * kk + h) & 3);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const int sb = (int)(h ? sc[t] >> 8 : sc[t]);
+          const int sw = (int)(s[h][t] >> shift);
 #pragma unroll
-          for (int u = 0; u < MT; ++u)
-            acc[u][t] = mfma_mx(wc[h][t], sb, x[u], (int)bc[h][u], acc[u][t]);
+          for (int u = 0; u < MT; ++u) acc[u][t] = mfma_mx(w[h][t], sw, x[u], sx[u], acc[u][t]);
         }
+        __builtin_amdgcn_sched_barrier(0);  // (or more operands than registers)
+        load(kk + 1, h);   // (past the last stage: its last columns once more, not used)
       }
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) keep(w[h][t], s[h][t]);   // (the waits above count every load)
+    wait_vm<0>();
     __syncthreads();
   }
 };

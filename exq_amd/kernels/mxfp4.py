@@ -14,9 +14,9 @@ import functools
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
-from .fused_moe import _check_routing
 from .linear import _ACTIVATIONS, _FLOAT_DTYPES, _GATED, _check_out, _layout, _overlap, _row_stride
 
 _BLOCK = 32
@@ -27,19 +27,20 @@ def _refuse_gradients(what, *tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{what} has no backward: call it under torch.no_grad()")
-    _lib.refuse_tangents(what, *tensors)
+    if forward_ad._current_level >= 0:
+        _lib.refuse_tangents(what, *tensors)
 
 
-def _device(*tensors) -> int:
+def _device(first, *others) -> int:
     """The index of the one HIP device that all tensors are on."""
-    first = tensors[0]
     dev = first.get_device()
-    for t in tensors:
-        if t is not None:
+    if dev < 0:
+        raise _lib.ExqError("exq_amd kernels need tensors on a HIP device (got CPU tensor)")
+    for t in others:
+        if t is not None and t.get_device() != dev:
             if t.get_device() < 0:
                 raise _lib.ExqError("exq_amd kernels need tensors on a HIP device (got CPU tensor)")
-            if t.get_device() != dev:
-                raise _lib.ExqError(f"tensors on different devices: {first.device} and {t.device}")
+            raise _lib.ExqError(f"tensors on different devices: {first.device} and {t.device}")
     return dev
 
 
@@ -63,18 +64,18 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     There is no derivative: an input that requires a gradient is refused unless
     gradients are off, and one with a forward-mode tangent always.
     """
-    if x.dim() < 1 or x.dtype not in _FLOAT_DTYPES:
+    shape = x.shape
+    if not shape or x.dtype not in _FLOAT_DTYPES:
         raise ValueError("x must be [.., K], float32, float16 or bfloat16")
-    K = x.shape[-1]
+    K = shape[-1]
     if K < _BLOCK or K % _BLOCK:
         raise ValueError(f"the last dimension must be a multiple of 32 (got {K})")
     _refuse_gradients("quantize_mxfp4", x)
     dev = _device(x)
-    shape = x.shape
-    if x.dim() != 2 or x.stride(1) != 1:
+    if len(shape) != 2 or x.stride(1) != 1:
         x = x.reshape(-1, K).contiguous()
-    packed = torch.empty(*shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(*shape[:-1], K // _BLOCK, dtype=torch.uint8, device=x.device)
+    packed = x.new_empty((*shape[:-1], K // 2), dtype=torch.uint8)
+    scales = x.new_empty((*shape[:-1], K // _BLOCK), dtype=torch.uint8)
     _lib.launch(_lib.lib().exq_quantize_mxfp4,
                 (x.data_ptr(), _lib._TORCH_TO_CODE[x.dtype], x.shape[0], K, x.stride(0),
                  packed.data_ptr(), scales.data_ptr()), dev, "quantize_mxfp4")
@@ -84,11 +85,10 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def _check_stored(packed, scales):
     if packed.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise ValueError("packed and scales must be uint8")
-    if (packed.dim() < 1 or packed.dim() != scales.dim() or packed.shape[-1] < 16
-            or packed.shape[-1] % 16 or packed.shape[:-1] != scales.shape[:-1]
-            or scales.shape[-1] * 16 != packed.shape[-1]):
-        raise ValueError(f"packed {tuple(packed.shape)} and scales {tuple(scales.shape)} must be "
-                         "[.., K/2] and [.., K/32], K a multiple of 32")
+    p, s = packed.shape, scales.shape
+    if not p or not s or p[-1] < 16 or p[-1] % 16 or p[:-1] != s[:-1] or s[-1] * 16 != p[-1]:
+        raise ValueError(f"packed {tuple(p)} and scales {tuple(s)} must be [.., K/2] and "
+                         "[.., K/32], K a multiple of 32")
 
 
 def dequantize_mxfp4(packed: torch.Tensor, scales: torch.Tensor,
@@ -101,8 +101,9 @@ def dequantize_mxfp4(packed: torch.Tensor, scales: torch.Tensor,
         raise ValueError("dtype must be float32, float16 or bfloat16")
     dev = _device(packed, scales)
     packed, scales = _aligned(packed), scales.contiguous()
-    K = packed.shape[-1] * 2
-    out = torch.empty(*packed.shape[:-1], K, dtype=dtype, device=packed.device)
+    shape = packed.shape
+    K = shape[-1] * 2
+    out = packed.new_empty((*shape[:-1], K), dtype=dtype)
     _lib.launch(_lib.lib().exq_dequantize_mxfp4,
                 (packed.data_ptr(), scales.data_ptr(), out.numel() // K, K, out.data_ptr(),
                  _lib._TORCH_TO_CODE[dtype]), dev, "dequantize_mxfp4")
@@ -179,10 +180,9 @@ def _check_weight(w, tiles, tile_scales, experts: bool):
             want *= n
 
 
-def _check_start(*tensors):
-    for t in tensors:
-        if t.data_ptr() % 16:
-            raise ValueError("tiles and tile_scales must start at a 16-byte address")
+def _check_start(address):
+    if address & 15:
+        raise ValueError("tiles and tile_scales must start at a 16-byte address")
 
 
 # ---- dense products ---------------------------------------------------------------------------
@@ -253,14 +253,13 @@ def _call(x, weight, bias, x_scales, activation, residual, out_dtype, out, gated
     p = _problem(_layout(x), *layouts)
     _refuse_gradients(what, x, bias, residual, out)
     dev = _device(x, tiles, tile_scales, bias, x_scales, residual, out)
-    _check_start(tiles, tile_scales)
+    _check_start(tiles.data_ptr() | tile_scales.data_ptr())
     if x.data_ptr() % 16 or (p.n_tokens > 1 and (p.x_stride * x.element_size() % 16
                                                  or p.x_stride > 1 << 22)):
         x = x.clone(memory_format=torch.contiguous_format)   # (rows at 16-byte addresses)
         p = _problem(_layout(x), *layouts)
     if out is None:
-        out = torch.empty(p.n_tokens, p.out_features, dtype=_OUT_DTYPES[p.out_dtype],
-                          device=x.device)
+        out = x.new_empty((p.n_tokens, p.out_features), dtype=_OUT_DTYPES[p.out_dtype])
     elif p.n_tokens:
         _check_out(p, out, x, tiles.view(-1, 1024), bias, residual)
         if _overlap(out, p.out_stride, tile_scales.view(-1, 256), 256) or (
@@ -316,30 +315,40 @@ def fused_gated_linear_mxfp4(x: torch.Tensor, weight: Mxfp4Weight,
 # ---- MoE layer --------------------------------------------------------------------------------
 
 @functools.lru_cache(maxsize=4096)
-def _moe_problem(hidden, w13, w2, weights, ids):
-    """(checked problem, workspace bytes) of a layer call, by its tensors' layouts."""
-    (shape, _, dtype), (ids_shape, _, ids_dtype) = hidden, ids
-    H, E = shape[1], w13[1][0][0]
-    if not w13[0][2] or w2[0][2]:
+def _moe_problem(shape, dtype, w13, w13_rest, w2, w2_rest, weights, weights_dtype, ids, ids_dtype):
+    """(checked problem, workspace bytes) of a layer call, by its tensors' shapes and types."""
+    if len(shape) != 2:
+        raise ValueError("hidden_states must be [T, H]")
+    if len(ids) != 2 or ids != weights or ids[0] != shape[0]:
+        raise ValueError("topk_ids / topk_weights must both be [T, k]")
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("hidden_states must be float16 or bfloat16")
+    if ids_dtype not in (torch.int32, torch.int64):
+        raise ValueError("topk_ids must be int32 or int64")
+    if weights_dtype not in _FLOAT_DTYPES:
+        raise ValueError("topk_weights must be float32, float16 or bfloat16")
+    (tiles13, scales13, rows13, cols13, gated13), (tiles2, scales2, rows2, cols2, gated2) = w13, w2
+    if not gated13 or gated2:
         raise ValueError("w13 must be a gated weight and w2 one that is not")
-    if len(w13[1][0]) != 5 or len(w2[1][0]) != 5 or w2[1][0][0] != E:
+    if len(tiles13) != 5 or len(tiles2) != 5 or tiles2[0] != tiles13[0]:
         raise ValueError("w13 and w2 must hold a weight for each expert, as many the one as the other")
-    _check_weight(*w13, True)
-    _check_weight(*w2, True)
-    I = w13[0][0] // 2
-    if w13[0][1] != H or w2[0][:2] != (H, I):
+    for w, (tiles_layout, scales_layout) in ((w13, w13_rest), (w2, w2_rest)):
+        _check_weight(w[2:], (w[0], *tiles_layout), (w[1], *scales_layout), True)
+    T, H, E, I = *shape, tiles13[0], rows13 // 2
+    if cols13 != H or (rows2, cols2) != (H, I):
         raise ValueError("the weights' sizes do not match hidden / intermediate sizes")
     code = _lib._TORCH_TO_CODE
-    p = _lib.MoeProblem(shape[0], H, I, E, ids_shape[1], 0, _BLOCK, code[dtype], code[ids_dtype],
-                        code[weights[2]])
+    p = _lib.MoeProblem(T, H, I, E, ids[1], 0, _BLOCK, code[dtype], code[ids_dtype],
+                        code[weights_dtype])
     need = _lib.lib().exq_moe_mxfp4_workspace_size(p)
-    if not need and shape[0]:
-        _lib.check(1, "fused_experts_mxfp4")
+    if not need:   # (the library's message: an argument out of its range)
+        raise _lib.ExqError(_lib.lib().exq_last_error().decode(errors="replace"))
     return p, need
 
 
-def _weight_layout(w: Mxfp4Weight):
-    return (w.rows, w.cols, w.gated), _layout(w.tiles), _layout(w.tile_scales)
+def _weight_key(w: Mxfp4Weight):
+    return ((w.tiles.shape, w.tile_scales.shape, w.rows, w.cols, w.gated),
+            ((w.tiles.stride(), w.tiles.dtype), (w.tile_scales.stride(), w.tile_scales.dtype)))
 
 
 def fused_experts_mxfp4(hidden_states: torch.Tensor, w13: Mxfp4Weight, w2: Mxfp4Weight,
@@ -361,13 +370,20 @@ def fused_experts_mxfp4(hidden_states: torch.Tensor, w13: Mxfp4Weight, w2: Mxfp4
     """
     if activation != "silu":
         raise ValueError(f"unsupported activation {activation!r} (only 'silu')")
-    _check_routing(hidden_states, topk_weights, topk_ids)
-    p, need = _moe_problem(_layout(hidden_states), _weight_layout(w13), _weight_layout(w2),
-                           _layout(topk_weights), _layout(topk_ids))
+    p, need = _moe_problem(hidden_states.shape, hidden_states.dtype, *_weight_key(w13),
+                           *_weight_key(w2), topk_weights.shape, topk_weights.dtype,
+                           topk_ids.shape, topk_ids.dtype)
     _refuse_gradients("fused_experts_mxfp4", hidden_states, topk_weights, out)
-    dev = _device(hidden_states, topk_weights, topk_ids, w13.tiles, w13.tile_scales, w2.tiles,
-                  w2.tile_scales, out, workspace)
-    _check_start(w13.tiles, w13.tile_scales, w2.tiles, w2.tile_scales)
+    tiles13, scales13, tiles2, scales2 = w13.tiles, w13.tile_scales, w2.tiles, w2.tile_scales
+    dev = _device(hidden_states, topk_weights, topk_ids, tiles13, scales13, tiles2, scales2, out,
+                  workspace)
+    if dev != torch._C._cuda_getDevice():   # (the stream and its capture are that device's)
+        with torch.cuda.device(dev):
+            return fused_experts_mxfp4(hidden_states, w13, w2, topk_weights, topk_ids, out=out,
+                                       workspace=workspace)
+    a13, b13, a2, b2 = (tiles13.data_ptr(), scales13.data_ptr(), tiles2.data_ptr(),
+                        scales2.data_ptr())
+    _check_start(a13 | b13 | a2 | b2)
     if not (hidden_states.is_contiguous() and topk_ids.is_contiguous()
             and topk_weights.is_contiguous()):
         raise _lib.ExqError("exq_amd kernels need contiguous tensors")
@@ -380,32 +396,34 @@ def fused_experts_mxfp4(hidden_states: torch.Tensor, w13: Mxfp4Weight, w2: Mxfp4
                              f"{hidden_states.dtype}")
         if not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("out must be contiguous and start at a 16-byte address")
-        for t in (hidden_states, topk_weights, topk_ids, w13.tiles, w13.tile_scales, w2.tiles,
-                  w2.tile_scales, workspace):
+        for t in (hidden_states, topk_weights, topk_ids, tiles13, scales13, tiles2, scales2,
+                  workspace):
             if t is not None and t.numel() and out.numel() and _overlap(
                     out.view(-1), out.numel(), t.view(-1), t.numel()):
                 raise ValueError("out overlaps an input")
     if p.n_tokens == 0:
         return out
     if workspace is None:
-        workspace = _scratch(out.device, dev, need)
+        workspace = _scratch(out, dev, need)
     elif (workspace.dtype != torch.uint8 or not workspace.is_contiguous()
           or workspace.data_ptr() % 16):
         raise ValueError("workspace must be contiguous uint8 and start at a 16-byte address")
     _lib.launch(_lib.lib().exq_moe_mxfp4_forward,
                 (p, hidden_states.data_ptr(), topk_ids.data_ptr(), topk_weights.data_ptr(),
-                 w13.tiles.data_ptr(), w13.tile_scales.data_ptr(), w2.tiles.data_ptr(),
-                 w2.tile_scales.data_ptr(), out.data_ptr(), workspace.data_ptr(),
-                 workspace.numel()), dev, "fused_experts_mxfp4")
+                 a13, b13, a2, b2, out.data_ptr(), workspace.data_ptr(), workspace.numel()), dev,
+                "fused_experts_mxfp4")
     return out
 
 
-def _scratch(device: torch.device, index: int, need: int) -> torch.Tensor:
-    """The workspace of the device's current stream; under capture memory of the graph's own,
-    as two graphs captured on one stream may be replayed at the same time."""
+def _scratch(out: torch.Tensor, index: int, need: int) -> torch.Tensor:
+    """The workspace of the current stream of out's device; under capture memory of the graph's
+    own, as two graphs captured on one stream may be replayed at the same time."""
     if torch._C._cuda_isCurrentStreamCapturing():
-        return torch.empty(need, dtype=torch.uint8, device=device)
-    return _lib.workspace(device, need, "mxfp4", torch._C._cuda_getCurrentRawStream(index))
+        return out.new_empty(need, dtype=torch.uint8)
+    ws = _lib._ws_cache.get((index, torch._C._cuda_getCurrentRawStream(index), "mxfp4"))
+    if ws is not None and ws.numel() >= need:
+        return ws
+    return _lib.workspace(out.device, need, "mxfp4")
 
 
 def moe_mxfp4_workspace_bytes(n_tokens: int, hidden: int, inter: int, n_experts: int,

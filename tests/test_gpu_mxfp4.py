@@ -420,6 +420,12 @@ LAYERS = [
     (4, 1024, 256, 128, 8), (7, 96, 544, 3, 2), (8, 256, 256, 16, 8), (16, 512, 192, 60, 4), (17, 128, 64, 2, 1),
     (33, 288, 160, 7, 3), (64, 512, 384, 128, 8), (64, 256, 256, 8, 2), (65, 256, 128, 16, 4), (100, 128, 1024, 4, 2),
     (187, 512, 224, 32, 8), (300, 256, 96, 8, 2), (513, 128, 128, 3, 1), (700, 96, 160, 40, 5), (1030, 64, 64, 9, 2),
+    # either side of 16, 32, 64, 128 and 512 slots and of 512 and 1,024 experts' routing
+    (16, 96, 64, 4, 1), (17, 96, 64, 4, 1), (2, 64, 64, 1024, 16), (3, 64, 64, 1024, 11), (64, 64, 32, 2, 1),
+    (65, 64, 32, 1024, 1), (128, 64, 64, 6, 1), (43, 64, 64, 512, 3), (64, 64, 96, 512, 8), (65, 96, 64, 64, 8),
+    (40, 64, 64, 600, 4), (129, 64, 32, 1024, 4), (1, 64, 64, 300, 64),
+    # 512 and more work-groups of each number of weight tiles a wave, and ragged last ones
+    (96, 1056, 160, 64, 4), (40, 2080, 1056, 8, 2), (200, 2048, 1056, 8, 2), (150, 4128, 96, 8, 2),
 ]
 
 

@@ -230,7 +230,13 @@ constexpr Shape kShapes[] = {
 constexpr const char* kKernels[] = {"stream 16x16", "stream 32x16", "tile 32x128", "tile 32x256",
                                     "tile 64x256",  "tile 128x256", "tile 256x256"};
 
-int pick_kernel(int64_t tokens, int64_t rows, bool x4, bool gated) {
+// `vec`: runs of the result and the residual may be stored and loaded at once.  Where they may
+// not, a tile's columns go one by one at its end, which the streams spread over more
+// work-groups (187 tokens x 1440 x 2047 with a residual: 32 x 128 tiles 15.7 us, 32 x 16
+// streams 12.3; x 2048 10.9 and 11.8).
+constexpr int kUnalignedTileNs = 5000;
+
+int pick_kernel(int64_t tokens, int64_t rows, int64_t KB, bool x4, bool gated, bool vec) {
   int best = 0;
   int64_t least = INT64_MAX;
   for (int i = 0; i < (int)(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {
@@ -239,7 +245,9 @@ int pick_kernel(int64_t tokens, int64_t rows, bool x4, bool gated) {
     if (ns[0] == 0) continue;
     const int64_t rows_of = gated && k.rows == 16 ? 32 : k.rows;
     const int64_t per_cu = cdiv(cdiv(tokens, k.tokens) * cdiv(rows, rows_of), 256);
-    const int64_t rest = per_cu % 3, t = per_cu / 3 * ns[2] + (rest ? ns[rest - 1] : 0);
+    const int64_t rest = per_cu % 3;
+    const int64_t t = (per_cu / 3 * ns[2] + (rest ? ns[rest - 1] : 0)) * KB +
+                      (vec || k.rows == 16 ? 0 : kUnalignedTileNs);
     if (t < least) {
       least = t;
       best = i;
@@ -250,7 +258,8 @@ int pick_kernel(int64_t tokens, int64_t rows, bool x4, bool gated) {
 
 template <bool BF, bool X4, bool GATED>
 int launch_products(const MxArgs& a, hipStream_t s) {
-  const int kernel = pick_kernel(a.T, a.N * (GATED ? 2 : 1), X4, GATED);
+  const int kernel = pick_kernel(a.T, a.N * (GATED ? 2 : 1), a.KB, X4, GATED,
+                                 a.vec_o && (a.vec_r || !a.res));
   switch (kernel) {
     case 0: return launch_stream<BF, X4, GATED, 1, 8>(a, s);
     case 1: return launch_stream<BF, X4, GATED, 2, 8>(a, s);
@@ -350,5 +359,6 @@ extern "C" int exq_linear_mxfp4(const exq_linear_problem* p, const void* x,
 extern "C" const char* exq_linear_mxfp4_kernel(const exq_linear_problem* p) {
   if (check_problem(p, nullptr, nullptr) != EXQ_SUCCESS || p->n_tokens == 0) return nullptr;
   return kKernels[pick_kernel(p->n_tokens, p->out_features * (p->gated ? 2 : 1),
-                              p->act_dtype == EXQ_DTYPE_U8, p->gated != 0)];
+                              mx::tile_cols(p->in_features), p->act_dtype == EXQ_DTYPE_U8,
+                              p->gated != 0, (p->out_stride | p->residual_stride) % 4 == 0)];
 }

@@ -577,7 +577,7 @@ int exq_stream_read(const void* buf, int64_t bytes, uint32_t* sink, int64_t sink
 const char* exq_linear_kernel(const exq_linear_problem* problem, const void* x,
                               const void* weight);
 
-/* The same for exq_linear_mxfp4 (the choice depends on the problem alone). */
+/* The same for exq_linear_mxfp4 with out and residual at 16-byte addresses. */
 const char* exq_linear_mxfp4_kernel(const exq_linear_problem* problem);
 
 #ifdef __cplusplus

@@ -212,7 +212,7 @@ def test_every_kernel_at_its_edges(x4, gated, kernel, T, N, K, device):
         X = torch.randint(-3, 4, (T, K), generator=torch.Generator().manual_seed(2)).double().cuda()
         x, x_scales = X.to(torch.bfloat16), None
     y = torch.mm(X, _dense(packed, scales).cuda().t())
-    hold = torch.full((T + 1, N + 3), 7.0, device="cuda")
+    hold = torch.full((T + 1, -(-N // 4) * 4 + 4), 7.0, device="cuda")
     if gated:
         fused_gated_linear_mxfp4(x, w, x_scales=x_scales, activation="relu", out=hold[:T, :N])
         want = (torch.relu(y[:, :N]) * y[:, N:]).float()

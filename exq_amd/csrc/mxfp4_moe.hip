@@ -262,8 +262,9 @@ int check_moe(const exq_moe_problem* p) {
               (long long)p->n_experts, (long long)k);
   EXQ_REQUIRE(p->n_shared == 0 && p->group_size == 32,
               "%s: no shared experts, and groups of 32", fn);
-  EXQ_REQUIRE_SUPPORTED(T * H <= ((int64_t)1 << 30) - 1, "%s: T=%lld x H=%lld: hidden is past 2 GiB",
-                        fn, (long long)T, (long long)H);
+  // (one buffer resource covers it: lin::kSpan bytes)
+  EXQ_REQUIRE_SUPPORTED(T <= (((int64_t)1 << 30) - 256) / H,
+                        "%s: T=%lld x H=%lld: hidden is past 2 GiB", fn, (long long)T, (long long)H);
   EXQ_REQUIRE_SUPPORTED(T <= ((int64_t)1 << 24) / k, "%s: T=%lld x k=%lld slots are too many", fn,
                         (long long)T, (long long)k);
   return EXQ_SUCCESS;

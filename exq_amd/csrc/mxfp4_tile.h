@@ -2,10 +2,12 @@
 // MoE kernels share.
 //
 // A work-group of WM x WN waves makes 16 MT WM tokens x 16 NT WN weight rows, a wave 16 MT
-// x 16 NT of them.  Tokens go through LDS, copied straight into one of two stages while
-// the other is multiplied; the waves meet once a stage.  Weights never do: a wave loads
-// its tiles of the next stage into registers, whole lines, a stage ahead, so LDS holds and
-// serves one operand only.
+// x 16 NT of them.  Tokens go through LDS, copied straight into one of its stages while
+// another is multiplied; the waves meet once a stage.  Weights never do: a wave loads its
+// tiles of the stages ahead into registers, whole lines, so LDS holds and serves one operand
+// only, and a decoded weight serves MT products.  Three work-groups a CU: 64 tokens x 256
+// rows reach what the library's bf16 product reaches (4096 x 4096 x 28672 1,355 TFLOP/s, the
+// library's 8192^3 1,390 on that card), two of 128 x 256 1,230, one of 256 x 256 1,044.
 //
 // LDS rows: a 16-bit stage is 128 columns, 256 bytes a row, sixteen 16-byte pieces; lane
 // (r, q) reads piece 4 q + j of its row for step j.  A ds_read_b128 is served 16 lanes at a
@@ -39,7 +41,7 @@ __device__ __forceinline__ void keep(const uint4& v, uint32_t s) {
 
 // Tokens of a work-group in 16 bits.  vo[j]: byte offset from xr's base of piece
 // `piece` of the row that the lane copies in copy j (kOob: none); a copy is four rows.
-// P stages: P - 1 are on their way while one is multiplied.
+// P >= 3 stages: P - 1 are on their way while one is multiplied.
 template <bool BF, int WM, int WN, int MT, int NT, int P>
 struct Tile16 {
   static constexpr int W = WM * WN;
@@ -49,7 +51,7 @@ struct Tile16 {
   static constexpr int LDS = P * STAGE;
   static constexpr int AHEAD = D + 2 * NT;                     // a wave's loads of a stage
   static_assert(BM % (4 * W) == 0 && W % 4 == 0 && LDS <= 160 * 1024, "copies");
-  static_assert((P - 1) * AHEAD < 64, "loads in flight");
+  static_assert(P >= 3 && (P - 1) * AHEAD < 64, "loads in flight");
 
   // Row of the work-group that the lane copies in copy j, and the piece of it.
   __device__ __forceinline__ static int row(int wave, int lane, int j) {
@@ -101,58 +103,36 @@ struct Tile16 {
       }
     };
     auto scale = [](uint32_t four, int kb) { return (four >> (8 * (kb & 3)) & 0xffu) << 23; };
-    if constexpr (P == 2) {
-      // (not unrolled by the stages: 236 registers, unrolled 409)
-      uint4 w[NT], wn[NT];
-      uint32_t s[NT], sn[NT];
-      copy(0, lds0);
-      load(0, wn, sn);
-      for (int kb = 0; kb < KB; ++kb) {
-        wait_vm<0>();
+    uint4 w[P][NT];
+    uint32_t s[P][NT];
+    // stage kb into place p; past the last one zeros, and its weights once more
+    auto fetch = [&](int kb, int p) {
+      copy(kb, lds0 + p * STAGE);
+      load(kb < KB ? kb : KB - 1, w[p], s[p]);
+    };
+#pragma unroll
+    for (int p = 0; p < P - 1; ++p) fetch(p, p);
+    for (int k0 = 0; k0 < KB; k0 += P) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const int kb = k0 + p;
+        if (p > 0 && kb >= KB) break;
+        wait_lds();   // (what the stage before read has arrived: its place is written next)
+        wait_vm<(P - 2) * AHEAD>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        uint32_t sc[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          w[t] = wn[t];
-          s[t] = scale(sn[t], kb);
-        }
-        if (kb + 1 < KB) {
-          copy(kb + 1, lds0 + ((kb + 1) & 1) * STAGE);
-          load(kb + 1, wn, sn);
-        }
-        multiply(lds + (kb & 1) * STAGE + rd, w, s);
+        for (int t = 0; t < NT; ++t) sc[t] = scale(s[p][t], kb);
+        fetch(kb + P - 1, (p + P - 1) % P);   // (over the stage that all have just left)
+        multiply(lds + p * STAGE + rd, w[p], sc);
       }
-    } else {
-      uint4 w[P][NT];
-      uint32_t s[P][NT];
-      // stage kb into place p; past the last one zeros, and its weights once more
-      auto fetch = [&](int kb, int p) {
-        copy(kb, lds0 + p * STAGE);
-        load(kb < KB ? kb : KB - 1, w[p], s[p]);
-      };
-#pragma unroll
-      for (int p = 0; p < P - 1; ++p) fetch(p, p);
-      for (int k0 = 0; k0 < KB; k0 += P) {
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-          const int kb = k0 + p;
-          if (p > 0 && kb >= KB) break;
-          wait_vm<(P - 2) * AHEAD>();
-          __builtin_amdgcn_s_barrier();
-          asm volatile("" ::: "memory");
-          uint32_t sc[NT];
-#pragma unroll
-          for (int t = 0; t < NT; ++t) sc[t] = scale(s[p][t], kb);
-          fetch(kb + P - 1, (p + P - 1) % P);   // (over the stage that all have just left)
-          multiply(lds + p * STAGE + rd, w[p], sc);
-        }
-      }
-      // (the waits above count every load: none may be dropped because no stage uses it)
-#pragma unroll
-      for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) keep(w[p][t], s[p][t]);
     }
+    // (the waits above count every load: none may be dropped because no stage uses it)
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) keep(w[p][t], s[p][t]);
     wait_vm<0>();
     __syncthreads();
   }

@@ -261,10 +261,10 @@ def _call(x, weight, bias, x_scales, activation, residual, out_dtype, out, gated
     if out is None:
         out = x.new_empty((p.n_tokens, p.out_features), dtype=_OUT_DTYPES[p.out_dtype])
     elif p.n_tokens:
-        _check_out(p, out, x, tiles.view(-1, 1024), bias, residual)
-        if _overlap(out, p.out_stride, tile_scales.view(-1, 256), 256) or (
-                x_scales is not None and _overlap(out, p.out_stride, x_scales, x_scales.shape[1])):
-            raise ValueError("out overlaps an input")
+        _check_out(p, out, x, tiles.view(1, -1), bias, residual)
+        for t in (tile_scales, x_scales):
+            if t is not None and _overlap(out, p.out_stride, t.view(1, -1), t.numel()):
+                raise ValueError("out overlaps an input")
     _lib.launch(_lib.lib().exq_linear_mxfp4,
                 (p, x.data_ptr(), None if x_scales is None else x_scales.data_ptr(),
                  tiles.data_ptr(), tile_scales.data_ptr(), None if bias is None else bias.data_ptr(),
@@ -399,15 +399,19 @@ def fused_experts_mxfp4(hidden_states: torch.Tensor, w13: Mxfp4Weight, w2: Mxfp4
         for t in (hidden_states, topk_weights, topk_ids, tiles13, scales13, tiles2, scales2,
                   workspace):
             if t is not None and t.numel() and out.numel() and _overlap(
-                    out.view(-1), out.numel(), t.view(-1), t.numel()):
+                    out.view(1, -1), out.numel(), t.view(1, -1), t.numel()):
                 raise ValueError("out overlaps an input")
     if p.n_tokens == 0:
         return out
     if workspace is None:
         workspace = _scratch(out, dev, need)
-    elif (workspace.dtype != torch.uint8 or not workspace.is_contiguous()
-          or workspace.data_ptr() % 16):
-        raise ValueError("workspace must be contiguous uint8 and start at a 16-byte address")
+    else:
+        if (workspace.dtype != torch.uint8 or not workspace.is_contiguous()
+                or workspace.data_ptr() % 16):
+            raise ValueError("workspace must be contiguous uint8 and start at a 16-byte address")
+        for t in (hidden_states, topk_weights, topk_ids, tiles13, scales13, tiles2, scales2):
+            if _overlap(workspace.view(1, -1), workspace.numel(), t.view(1, -1), t.numel()):
+                raise ValueError("workspace overlaps an input")
     _lib.launch(_lib.lib().exq_moe_mxfp4_forward,
                 (p, hidden_states.data_ptr(), topk_ids.data_ptr(), topk_weights.data_ptr(),
                  a13, b13, a2, b2, out.data_ptr(), workspace.data_ptr(), workspace.numel()), dev,

@@ -506,7 +506,8 @@ int exq_moe_mixed_forward(const exq_moe_problem* problem, const void* hidden,
  * zeros).  w13 [E, 2I, H] gated and w2 [E, H, I] in the order of tiles; weight values
  * take hidden's type as in exq_linear_mxfp4, silu(gate) * up is rounded to it, sums are
  * in fp32, and the k results of a token are added in a fixed order.  H and I are
- * multiples of 32, n_experts <= 1024, top_k <= 64, at most 2^24 slots; group_size is 32
+ * multiples of 32, n_experts <= 1024, top_k <= 64, at most 2^24 slots and 2 GiB of
+ * hidden (n_tokens * hidden_size <= 2^30 - 256); group_size is 32
  * and n_shared 0.  Pointers are 16-byte aligned.  The workspace needs no fill and must
  * not be shared by calls that may run concurrently.  No counterpart in the reference.
  */

@@ -316,6 +316,30 @@ def test_strides_and_neighbours(T, kind, device):
     assert fused_linear_mxfp4(x[:0], w, x_scales=None if x_scales is None else x_scales[:0]).shape == (0, N)
 
 
+def test_overlaps_are_refused(device):
+    """out anywhere in an input but the residual, a workspace in the layer's inputs."""
+    from exq_amd.kernels import Mxfp4Weight, fused_experts_mxfp4, fused_linear_mxfp4
+    T, K, N = 8, 256, 64
+    packed, scales = _codes(N, K, 1, 0, 0)
+    w = Mxfp4Weight.from_packed(packed.cuda(), scales.cuda())
+    x = torch.ones(T, K, dtype=torch.bfloat16).cuda()
+    tail = w.tiles.view(-1)[-2 * T * N:].view(torch.bfloat16).view(T, N)
+    wide = Mxfp4Weight(w.tiles, torch.zeros(2 * T * N, dtype=torch.uint8).cuda()[:w.tile_scales.numel()]
+                       .view(w.tile_scales.shape), N, K)
+    in_scales = wide.tile_scales.view(-1)[:2 * 4 * N].view(torch.bfloat16).view(4, N)
+    xp, xs = (t.cuda() for t in _codes(64, K, 2, 0, 0))
+    for call in (lambda: fused_linear_mxfp4(x, w, out=tail),
+                 lambda: fused_linear_mxfp4(x[:4], wide, out=in_scales),
+                 lambda: fused_linear_mxfp4(x, w, out=x[:, :N]),
+                 lambda: fused_linear_mxfp4(xp[:1], w, x_scales=xs[:1], out=xp[:1, :N * 2].view(torch.bfloat16)),
+                 lambda: fused_linear_mxfp4(x, w, residual=x[:, :N], out=x[:, 1:N + 1])):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    h, _, _, w13, w2, ids, wts = _layer(4, 64, 64, 4, 2, torch.bfloat16, 1)
+    with pytest.raises(ValueError, match="workspace overlaps"):
+        fused_experts_mxfp4(h, w13, w2, wts, ids, workspace=w13.tiles.view(-1))
+
+
 @pytest.mark.parametrize("T", [3, 70, 300])
 @pytest.mark.parametrize("kind", ["bf16", "x4"])
 def test_nan_and_infinity_stay_in_their_row_and_column(T, kind, device):
@@ -541,6 +565,25 @@ def test_block(T, device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(captured, want)
+
+
+@pytest.mark.parametrize("T", [1, 3, 30, 90])
+def test_two_streams_at_once(T, device):
+    """Calls in flight on two streams: a workspace each."""
+    from exq_amd.kernels import fused_experts_mxfp4
+    a = _layer(T, 512, 256, 16, 4, torch.bfloat16, 1)
+    b = _layer(T, 512, 256, 16, 4, torch.bfloat16, 2)
+    want = [fused_experts_mxfp4(x, w13, w2, w, ids) for x, _, _, w13, w2, ids, w in (a, b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(10):
+        for i, (x, _, _, w13, w2, ids, w) in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(fused_experts_mxfp4(x, w13, w2, w, ids))
+    torch.cuda.synchronize()
+    for got, ref in zip(outs, want):
+        assert all(torch.equal(o, ref) for o in got)
 
 
 def test_two_graphs_at_once(device):

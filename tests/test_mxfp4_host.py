@@ -159,6 +159,8 @@ def test_library_refusals():
         need, status = moe(**bad)
         assert need == 0 and status == 1, bad
     assert moe(n_tokens=1 << 24)[1] == 2           # slots
+    assert moe(n_tokens=1 << 22, hidden_size=256, top_k=1)[1] == 2   # hidden past 2 GiB
+    assert moe(n_tokens=(1 << 22) - 1, hidden_size=256, top_k=1)[1] == 3
     assert L.exq_quantize_mxfp4(one, _lib.F32, 1, 48, 48, one, one, None) == 1
     assert L.exq_quantize_mxfp4(one, _lib.I32, 1, 64, 64, one, one, None) == 1
     assert L.exq_quantize_mxfp4(one, _lib.F32, 0, 64, 64, None, None, None) == 0

@@ -20,18 +20,12 @@ namespace mx {
 
 constexpr int kBlock = 32;          // values of a block
 constexpr int kTileK = 128;         // columns of a tile
-constexpr int kTileBytes = 1024;
 
 inline int64_t tile_cols(int64_t K) { return cdiv(K, kTileK); }
 // Tiles of rows of a weight; a gated one (gate rows, then up rows) pads each half and
 // has its gate and up tiles in turn.
 inline int64_t tile_rows(int64_t rows, int gated) {
   return gated ? 2 * cdiv(rows / 2, 16) : cdiv(rows, 16);
-}
-
-// The scale of byte i of four scale bytes, as the conversions take it.
-__device__ __forceinline__ float scale_of(uint32_t four, int i) {
-  return __uint_as_float(i == 3 ? (four >> 1) & 0x7f800000u : ((four >> (8 * i)) & 0xffu) << 23);
 }
 
 // Eight codes times the scale, in 16 bits: exact in bf16 but past its largest value, in

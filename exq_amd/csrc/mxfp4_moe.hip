@@ -1,5 +1,18 @@
 // mxfp4_moe.hip -- the MoE layer with MXFP4 experts:
 //   out[t] = sum_j w[t, j] * W2_e (silu(Wg_e x_t) * (Wu_e x_t)),  e = ids[t, j]
+//
+// Few slots are bound by the latency of a chain of kernels and by the active experts' bytes,
+// many by the matrix instructions, so the number of slots n = T k says which kernels run
+// (path_of):
+//   n <= kSlotSlots    a slot is a group: two kernels, no routing (1 token x 8 of 128 experts of
+//                      2048 x 768 13.6 us a call)
+//   n <= kOwnedSlots   gate/up tiles route, the down kernel sums all slots of its columns
+//   n <= 512           gate/up tiles route, down tiles write fp32 rows, a third kernel adds a
+//                      token's (64 tokens 50 us, floor 26; 16 x 8 of 64 of 2048 x 1024 34 - 42, 21)
+//   more               the plan is made first (2001 tokens x 6 of 64 of 2048 x 1408 251 us, floor
+//                      149 at the rate of a large bf16 product; the plan 15, the sums 27)
+// mid = silu(gate) * up is rounded to the activations' type, which the second product's matrix
+// instructions take; all sums are in 32 bits, each in a fixed order.
 #include "mxfp4_route.h"
 #include "mxfp4_stream.h"
 

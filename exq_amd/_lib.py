@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import threading
+import weakref
 from pathlib import Path
 
 import torch
@@ -203,29 +204,54 @@ def require_gpu(*tensors: torch.Tensor) -> torch.device:
     return None if first is None else first.device
 
 
-# Per-(device, stream, kind) workspace cache: reused across calls on one
-# stream, which is safe because launches on one stream are ordered.  The
-# fused-layer workspace ("fused") is kept apart from the scratch of the other
-# entry points (its first bytes hold the decode kernels' combine counters,
-# which each fused call clears itself).
-_ws_cache: dict[tuple[int, int, str], torch.Tensor] = {}
+class _Buffers:
+    """One thread's workspaces by (device, stream, kind)."""
+
+    def __init__(self):
+        self.by_key: dict[tuple[int, int, str], torch.Tensor] = {}
+
+
+_all_buffers: weakref.WeakSet = weakref.WeakSet()
+
+
+class _Workspaces(threading.local):
+    """The calling thread's own workspaces, reused across its calls on one stream, whose
+    launches are ordered.  A call is several launches that hand their results over in the
+    workspace, and ctypes lets go of the GIL for it: another thread's call on the same
+    stream (by default all threads share one) may be enqueued between them, so it works
+    in another buffer.  A thread's buffers end with it.  The fused-layer workspace
+    ("fused") is kept apart from the scratch of the other entry points (its first bytes
+    hold the decode kernels' combine counters, which each fused call clears itself)."""
+
+    def __init__(self):
+        self.buffers = _Buffers()
+        with _lock:
+            _all_buffers.add(self.buffers)
+
+
+_workspaces = _Workspaces()
 
 
 def workspace(device: torch.device, nbytes: int, kind: str = "scratch",
               stream: int | None = None) -> torch.Tensor:
-    """The workspace of ``kind`` for the device's current stream (``stream``: its
-    handle, where the caller has it already)."""
+    """The calling thread's workspace of ``kind`` for the device's current stream
+    (``stream``: its handle, where the caller has it already)."""
     key = (device.index if device.index is not None else torch.cuda.current_device(),
            stream_handle(device) if stream is None else stream, kind)
-    buf = _ws_cache.get(key)
+    buffers = _workspaces.buffers.by_key
+    buf = buffers.get(key)
     if buf is None or buf.numel() < nbytes:
         size = max(nbytes, 1 << 20)
         if buf is not None:
             size = max(size, buf.numel() * 3 // 2)
         buf = torch.zeros(size, dtype=torch.uint8, device=device)
-        _ws_cache[key] = buf
+        buffers[key] = buf
     return buf
 
 
 def clear_workspace_cache() -> None:
-    _ws_cache.clear()
+    """Let go of every thread's workspaces."""
+    with _lock:
+        every = list(_all_buffers)
+    for buffers in every:
+        buffers.by_key.clear()

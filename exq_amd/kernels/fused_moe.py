@@ -94,10 +94,10 @@ def fused_experts(hidden_states: torch.Tensor, w13_packed: torch.Tensor,
     topk_weights [T, k] f32/f16/bf16; topk_ids [T, k] i32/i64 (ids outside
     [0, E) are dropped).  Returns [T, H] in the activation dtype.  The call is
     stream-ordered and never synchronises with the host.  ``workspace`` (uint8,
-    at least ``moe_workspace_bytes(...)``) replaces the per-stream cached one,
-    e.g. for HIP-graph capture; any contents will do (``torch.empty``), since
-    each call's first kernel clears the counters its first bytes hold, but it
-    must not be shared by calls that may run concurrently.
+    at least ``moe_workspace_bytes(...)``) replaces the one that each thread keeps
+    for a stream, e.g. for HIP-graph capture; any contents will do
+    (``torch.empty``), since each call's first kernel clears the counters its
+    first bytes hold, but it must not be shared by calls that may run concurrently.
     """
     if activation != "silu":
         raise ValueError(f"unsupported activation {activation!r} (only 'silu')")

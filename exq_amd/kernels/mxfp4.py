@@ -365,8 +365,8 @@ def fused_experts_mxfp4(hidden_states: torch.Tensor, w13: Mxfp4Weight, w2: Mxfp4
     ``fused_linear_mxfp4``; ``silu(gate) * up`` is rounded to it, as in ``fused_experts``.
     Stream-ordered, no synchronisation with the host.  ``workspace``: uint8, at least
     ``moe_mxfp4_workspace_bytes(...)``, not shared by calls that may run at once;
-    without one the call uses the stream's own, and under graph capture one of the
-    graph's.  ``out`` must not overlap an input.  No derivative.
+    without one the call uses the calling thread's for the stream, and under graph
+    capture one of the graph's.  ``out`` must not overlap an input.  No derivative.
     """
     if activation != "silu":
         raise ValueError(f"unsupported activation {activation!r} (only 'silu')")
@@ -420,14 +420,11 @@ def fused_experts_mxfp4(hidden_states: torch.Tensor, w13: Mxfp4Weight, w2: Mxfp4
 
 
 def _scratch(out: torch.Tensor, index: int, need: int) -> torch.Tensor:
-    """The workspace of the current stream of out's device; under capture memory of the graph's
-    own, as two graphs captured on one stream may be replayed at the same time."""
+    """The thread's workspace for the current stream of out's device; under capture memory of
+    the graph's own, as two graphs captured on one stream may be replayed at the same time."""
     if torch._C._cuda_isCurrentStreamCapturing():
         return out.new_empty(need, dtype=torch.uint8)
-    ws = _lib._ws_cache.get((index, torch._C._cuda_getCurrentRawStream(index), "mxfp4"))
-    if ws is not None and ws.numel() >= need:
-        return ws
-    return _lib.workspace(out.device, need, "mxfp4")
+    return _lib.workspace(out.device, need, "mxfp4", torch._C._cuda_getCurrentRawStream(index))
 
 
 def moe_mxfp4_workspace_bytes(n_tokens: int, hidden: int, inter: int, n_experts: int,

@@ -232,10 +232,24 @@ class _Workspaces(threading.local):
 _workspaces = _Workspaces()
 
 
+def _capturing(device: torch.device) -> bool:
+    """Whether the device's current stream is being captured into a graph."""
+    if device.type != "cuda":
+        return False
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return torch._C._cuda_isCurrentStreamCapturing()
+    with torch.cuda.device(device):
+        return torch._C._cuda_isCurrentStreamCapturing()
+
+
 def workspace(device: torch.device, nbytes: int, kind: str = "scratch",
               stream: int | None = None) -> torch.Tensor:
     """The calling thread's workspace of ``kind`` for the device's current stream
-    (``stream``: its handle, where the caller has it already)."""
+    (``stream``: its handle, where the caller has it already).  Under capture memory of the
+    graph's own: a graph is replayed at the same time as others that were captured on its
+    stream, and after a larger call has let go of a buffer that it holds the address of."""
+    if _capturing(device):
+        return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
     key = (device.index if device.index is not None else torch.cuda.current_device(),
            stream_handle(device) if stream is None else stream, kind)
     buffers = _workspaces.buffers.by_key

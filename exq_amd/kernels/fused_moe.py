@@ -95,8 +95,8 @@ def fused_experts(hidden_states: torch.Tensor, w13_packed: torch.Tensor,
     [0, E) are dropped).  Returns [T, H] in the activation dtype.  The call is
     stream-ordered and never synchronises with the host.  ``workspace`` (uint8,
     at least ``moe_workspace_bytes(...)``) replaces the one that each thread keeps
-    for a stream, e.g. for HIP-graph capture; any contents will do
-    (``torch.empty``), since each call's first kernel clears the counters its
+    for a stream (under graph capture one of the graph's own); any contents will
+    do (``torch.empty``), since each call's first kernel clears the counters its
     first bytes hold, but it must not be shared by calls that may run concurrently.
     """
     if activation != "silu":

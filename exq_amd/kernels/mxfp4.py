@@ -404,7 +404,8 @@ def fused_experts_mxfp4(hidden_states: torch.Tensor, w13: Mxfp4Weight, w2: Mxfp4
     if p.n_tokens == 0:
         return out
     if workspace is None:
-        workspace = _scratch(out, dev, need)
+        workspace = _lib.workspace(out.device, need, "mxfp4",
+                                   torch._C._cuda_getCurrentRawStream(dev))
     else:
         if (workspace.dtype != torch.uint8 or not workspace.is_contiguous()
                 or workspace.data_ptr() % 16):
@@ -417,14 +418,6 @@ def fused_experts_mxfp4(hidden_states: torch.Tensor, w13: Mxfp4Weight, w2: Mxfp4
                  a13, b13, a2, b2, out.data_ptr(), workspace.data_ptr(), workspace.numel()), dev,
                 "fused_experts_mxfp4")
     return out
-
-
-def _scratch(out: torch.Tensor, index: int, need: int) -> torch.Tensor:
-    """The thread's workspace for the current stream of out's device; under capture memory of
-    the graph's own, as two graphs captured on one stream may be replayed at the same time."""
-    if torch._C._cuda_isCurrentStreamCapturing():
-        return out.new_empty(need, dtype=torch.uint8)
-    return _lib.workspace(out.device, need, "mxfp4", torch._C._cuda_getCurrentRawStream(index))
 
 
 def moe_mxfp4_workspace_bytes(n_tokens: int, hidden: int, inter: int, n_experts: int,

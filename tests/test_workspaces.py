@@ -71,3 +71,14 @@ def test_clearing_reaches_every_thread():
     mine = _lib.workspace(CPU, 100, "fused", 7)
     _in_thread(_lib.clear_workspace_cache)
     assert _lib.workspace(CPU, 100, "fused", 7) is not mine
+
+
+def test_a_graph_has_workspaces_of_its_own(monkeypatch):
+    """Two graphs captured on one stream may run at once, and a buffer whose address a graph
+    holds must not be let go of when a later call needs a larger one."""
+    eager = _lib.workspace(CPU, 100, "fused", 7)
+    monkeypatch.setattr(_lib, "_capturing", lambda device: True)
+    graphs = [_lib.workspace(CPU, 100, "fused", 7) for _ in range(2)]
+    assert len({t.data_ptr() for t in (eager, *graphs)}) == 3
+    monkeypatch.undo()
+    assert _lib.workspace(CPU, 100, "fused", 7) is eager

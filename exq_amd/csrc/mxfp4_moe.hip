@@ -326,7 +326,7 @@ extern "C" int exq_moe_mxfp4_forward(const exq_moe_problem* p, const void* hidde
   a.mid = reinterpret_cast<uint16_t*>(ws + l.mid);
   a.part = reinterpret_cast<float*>(ws + l.part);
   if (!r.by_slot && r.nseg == 0) {
-    RoutePlanParams rp{};
+    RoutePlanParams rp{};   // (no rp.out: the combine kernel writes all of it, zeros too)
     rp.ids = topk_ids;
     rp.ids_dtype = p->ids_dtype;
     rp.T = (int)T;
@@ -341,8 +341,6 @@ extern "C" int exq_moe_mxfp4_forward(const exq_moe_problem* p, const void* hidde
     rp.tg_cap = (int)l.tg_cap;
     rp.i4_group = rp.bf_group = rp.i8_group = rp.i4_big_group = kTileGroup;
     rp.i4_big_rows = kTileGroup / 2 + 1;   // (the groups that take longest first)
-    rp.out = out;
-    rp.out_bytes = T * H * 2;
     rp.blk_cnt = reinterpret_cast<int*>(ws + l.blk);
     st = launch_route_plan(rp, s);
     if (st) return st;

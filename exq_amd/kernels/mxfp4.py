@@ -284,9 +284,10 @@ def fused_linear_mxfp4(x: torch.Tensor, weight: Mxfp4Weight, bias: torch.Tensor 
     [T, K/2] packed with ``x_scales`` [T, K/32], as ``quantize_mxfp4`` gives them: both
     operands go to the 4-bit matrix instructions.  bias, residual, ``activation`` and
     ``out`` as in ``fused_linear``; returns [T, N] in ``out_dtype`` (default x's,
-    bfloat16 for packed x).  Sums in float32, one rounding at the end.  x's row stride
-    is free; rows that do not start at 16-byte addresses, or lie more than 2^22
-    elements apart, are copied first.
+    bfloat16 for packed x).  Sums in float32, one rounding at the end; the 4-bit
+    instructions, which add 128 products and the sum so far at once, drop what lies more
+    than 2^23 below the largest of them.  x's row stride is free; rows that do not start
+    at 16-byte addresses, or lie more than 2^22 elements apart, are copied first.
     Stream-ordered, graph-capturable, no workspace, no derivative (as ``fused_linear``).
     """
     if activation not in _ACTIVATIONS:
@@ -362,7 +363,9 @@ def fused_experts_mxfp4(hidden_states: torch.Tensor, w13: Mxfp4Weight, w2: Mxfp4
     w2 of [E, H, I]; topk_weights [T, k] float32 / float16 / bfloat16; topk_ids [T, k]
     int32 / int64 (ids outside [0, E) are dropped; a token without experts gets zeros).
     Returns [T, H] in hidden's type.  The weights' values take hidden's type as in
-    ``fused_linear_mxfp4``; ``silu(gate) * up`` is rounded to it, as in ``fused_experts``.
+    ``fused_linear_mxfp4``; ``silu(gate) * up`` is rounded to it, as in ``fused_experts``
+    (in float16 it becomes infinite past 65504), for the second product's matrix
+    instructions, which take two operands of one type.
     Stream-ordered, no synchronisation with the host.  ``workspace``: uint8, at least
     ``moe_mxfp4_workspace_bytes(...)``, not shared by calls that may run at once;
     without one the call uses the calling thread's for the stream, and under graph

@@ -360,8 +360,10 @@ int exq_tile_mxfp4(const uint8_t* packed, const uint8_t* scales, int64_t n_matri
  * x [T, K] is 16-bit and the weight's values take its type, exact in bf16, rounded to
  * nearest in f16 (exact for scales 2^-23 .. 2^13); x_scales is not read.  act_dtype u8: x
  * [T, K/2] is MXFP4 too, x_stride bytes from row to row, with x_scales [T, K/32].
- * Products are summed in fp32 and the result is rounded once, to out_dtype.  x's rows
- * (at most 2^22 elements apart), tiles and tile_scales are 16-byte aligned; K <= 2^22.  out may be residual itself (same pointer,
+ * Products are summed in fp32 and the result is rounded once, to out_dtype; with MXFP4 x
+ * an instruction, which adds 128 products and the sum so far, drops what lies more than
+ * 2^23 below the largest of them.  x's rows (at most 2^22 elements apart), tiles and
+ * tile_scales are 16-byte aligned; K <= 2^22.  out may be residual itself (same pointer,
  * dtype and stride) and must not overlap any other input.  No workspace.
  */
 int exq_linear_mxfp4(const exq_linear_problem* problem, const void* x, const uint8_t* x_scales,
@@ -504,8 +506,8 @@ int exq_moe_mixed_forward(const exq_moe_problem* problem, const void* hidden,
  * The MoE layer with MXFP4 experts: out[t] = sum_j w[t, j] * W2 (silu(Wg x_t) * Wu x_t)
  * of expert ids[t, j], ids outside [0, n_experts) dropped (a token without experts gets
  * zeros).  w13 [E, 2I, H] gated and w2 [E, H, I] in the order of tiles; weight values
- * take hidden's type as in exq_linear_mxfp4, silu(gate) * up is rounded to it, sums are
- * in fp32, and the k results of a token are added in a fixed order.  H and I are
+ * take hidden's type as in exq_linear_mxfp4, silu(gate) * up is rounded to it (in f16
+ * infinite past 65504), sums are in fp32, and the k results of a token are added in a fixed order.  H and I are
  * multiples of 32, n_experts <= 1024, top_k <= 64, at most 2^24 slots and 2 GiB of
  * hidden (n_tokens * hidden_size <= 2^30 - 256); group_size is 32
  * and n_shared 0.  Pointers are 16-byte aligned.  The workspace needs no fill and must

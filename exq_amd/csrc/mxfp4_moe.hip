@@ -4,9 +4,8 @@
 // Few slots are bound by the latency of a chain of kernels and by the active experts' bytes,
 // many by the matrix instructions, so the number of slots n = T k says which kernels run
 // (path_of):
-//   n <= kSlotSlots    a slot is a group: two kernels, no routing (1 token x 8 of 128 experts of
-//                      2048 x 768 13.6 us a call)
-//   n <= kOwnedSlots   gate/up tiles route, the down kernel sums all slots of its columns
+//   few (runs_by_slot) a slot is a group: two kernels, no routing, the second one sums all
+//                      slots of its columns (1 token x 8 of 128 experts of 2048 x 768 13.6 us)
 //   n <= 512           gate/up tiles route, down tiles write fp32 rows, a third kernel adds a
 //                      token's (64 tokens 50 us, floor 26; 16 x 8 of 64 of 2048 x 1024 34 - 42, 21)
 //   more               the plan is made first (2001 tokens x 6 of 64 of 2048 x 1408 251 us, floor
@@ -98,8 +97,8 @@ __device__ __forceinline__ void moe_tile(const MoeArgs& a, unsigned char* lds, c
       });
 }
 
-// NSEG > 0: the kernel routes (gate/up), the plan in groups of PLAN rows.
-template <bool BF, bool GATEUP, int NT, int NSEG, int PLAN>
+// NSEG > 0: the kernel routes (gate/up).
+template <bool BF, bool GATEUP, int NT, int NSEG>
 __global__ void __launch_bounds__(256, 3) moe_tile_kernel(MoeArgs a, RouteArgs ra, int n_tiles) {
   __shared__ __align__(1024) unsigned char lds[kTileLds];
   int tgi, nb;
@@ -110,7 +109,7 @@ __global__ void __launch_bounds__(256, 3) moe_tile_kernel(MoeArgs a, RouteArgs r
     __shared__ TgEntry own;
     __shared__ int rows[kTileGroup];
     static_assert(R::kWords * 4 <= kTileLds && kTileGroup == 64, "routing scratch");
-    if (!R::template here<PLAN>(ra, reinterpret_cast<uint32_t*>(lds), &own, rows, [&](int n) {
+    if (!R::here(ra, reinterpret_cast<uint32_t*>(lds), &own, rows, [&](int n) {
           return spread_unit(blockIdx.x, n, n_tiles, tgi, nb) ? tgi : -1;
         }))
       return;
@@ -190,35 +189,32 @@ int launch_moe_tile(Kernel kernel, const MoeArgs& a, const RouteArgs& ra, int64_
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, s, a, ra, (int)n_tiles);
   return check_launch("moe_tile_kernel");
 }
-template <bool BF, int NSEG, int PLAN>
+template <bool BF, int NSEG>
 int launch_gateup_as(const MoeArgs& a, const RouteArgs& ra, hipStream_t s) {
   const int64_t groups = tg_capacity(ra.n, ra.E, kTileGroup);
   if (wave_tiles(groups, a.RT, 2) == 4)
-    return launch_moe_tile(moe_tile_kernel<BF, true, 4, NSEG, PLAN>, a, ra, groups, 4, s);
-  return launch_moe_tile(moe_tile_kernel<BF, true, 2, NSEG, PLAN>, a, ra, groups, 2, s);
+    return launch_moe_tile(moe_tile_kernel<BF, true, 4, NSEG>, a, ra, groups, 4, s);
+  return launch_moe_tile(moe_tile_kernel<BF, true, 2, NSEG>, a, ra, groups, 2, s);
 }
 template <bool BF>
 int launch_down(const MoeArgs& a, int64_t groups, hipStream_t s) {
   switch (wave_tiles(groups, a.RT, 1)) {
-    case 4: return launch_moe_tile(moe_tile_kernel<BF, false, 4, 0, 64>, a, RouteArgs{}, groups, 4, s);
-    case 2: return launch_moe_tile(moe_tile_kernel<BF, false, 2, 0, 64>, a, RouteArgs{}, groups, 2, s);
-    default: return launch_moe_tile(moe_tile_kernel<BF, false, 1, 0, 64>, a, RouteArgs{}, groups, 1, s);
+    case 4: return launch_moe_tile(moe_tile_kernel<BF, false, 4, 0>, a, RouteArgs{}, groups, 4, s);
+    case 2: return launch_moe_tile(moe_tile_kernel<BF, false, 2, 0>, a, RouteArgs{}, groups, 2, s);
+    default: return launch_moe_tile(moe_tile_kernel<BF, false, 1, 0>, a, RouteArgs{}, groups, 1, s);
   }
 }
 
-// How a batch runs: which kernels route, make the partial rows and add them.
+// How a batch runs.
 struct Path {
   int64_t n;       // slots
-  bool by_slot;    // gate/up by slots, no routing
-  bool owned;      // down by output columns, no partial rows
+  bool by_slot;    // no routing, down by output columns without partial rows
   int nseg;        // the gate/up tiles route, 64 nseg slots at most; 0: a plan kernel first
 };
 Path path_of(const exq_moe_problem* p) {
-  static_assert(kSlotSlots <= kOwnedSlots && kOwnedSlots <= 64, "paths");
   Path r;
   r.n = p->n_tokens * p->top_k;
-  r.owned = r.n <= kOwnedSlots;
-  r.by_slot = r.n <= kSlotSlots;
+  r.by_slot = runs_by_slot(r.n, p->hidden_size, p->inter_size);
   r.nseg = r.by_slot ? 0 : r.n <= 64 ? 1 : r.n <= 128 ? 2
            : r.n <= 512 && p->n_experts <= Router<8>::kExperts ? 8 : 0;
   return r;
@@ -226,12 +222,11 @@ Path path_of(const exq_moe_problem* p) {
 
 template <bool BF>
 int launch_gateup(const MoeArgs& a, const RouteArgs& ra, const Path& r, hipStream_t s) {
-  if (r.owned) return launch_gateup_as<BF, 1, 16>(a, ra, s);   // (owned slots fit one segment)
   switch (r.nseg) {
-    case 1: return launch_gateup_as<BF, 1, 64>(a, ra, s);
-    case 2: return launch_gateup_as<BF, 2, 64>(a, ra, s);
-    case 8: return launch_gateup_as<BF, 8, 64>(a, ra, s);
-    default: return launch_gateup_as<BF, 0, 64>(a, ra, s);
+    case 1: return launch_gateup_as<BF, 1>(a, ra, s);
+    case 2: return launch_gateup_as<BF, 2>(a, ra, s);
+    case 8: return launch_gateup_as<BF, 8>(a, ra, s);
+    default: return launch_gateup_as<BF, 0>(a, ra, s);
   }
 }
 
@@ -248,14 +243,14 @@ Layout layout(const exq_moe_problem* p) {
     at = align_up(at + bytes, 256);
     return o;
   };
-  l.tg_cap = tg_capacity(r.n, p->n_experts, r.owned ? 16 : kTileGroup);
+  l.tg_cap = tg_capacity(r.n, p->n_experts, kTileGroup);
   l.hdr = take(64);
   l.tg = take((size_t)l.tg_cap * sizeof(TgEntry));
   l.sorted = take((size_t)r.n * 4);
   l.ends = take((size_t)(p->n_experts + 1) * 4);
   l.blk = take((size_t)route_plan_blocks(r.n) * p->n_experts * 4);
   l.mid = take((size_t)r.n * p->inter_size * 2);
-  l.part = take(r.owned ? 0 : (size_t)r.n * p->hidden_size * 4);
+  l.part = take(r.by_slot ? 0 : (size_t)r.n * p->hidden_size * 4);
   l.total = at;
   return l;
 }
@@ -372,11 +367,10 @@ extern "C" int exq_moe_mxfp4_forward(const exq_moe_problem* p, const void* hidde
   if (st) return st;
   weights_of(w2_tiles, w2_scales, I, H, H, 0);
   a.x = a.mid;
-  if (r.owned) {
-    const OwnedArgs o{r.by_slot ? nullptr : a.hdr, a.tg, a.sorted, a.mid, a.tiles,
-                      reinterpret_cast<const uint8_t*>(a.wscales), topk_ids, topk_weights,
-                      p->ids_dtype, p->weights_dtype, (int)T, k, E, (int)I, (int)H, a.KB, a.G,
-                      a.RT, reinterpret_cast<uint16_t*>(out)};
+  if (r.by_slot) {
+    const OwnedArgs o{a.mid, a.tiles, reinterpret_cast<const uint8_t*>(a.wscales), topk_ids,
+                      topk_weights, p->ids_dtype, p->weights_dtype, (int)T, k, E, (int)I, (int)H,
+                      a.KB, a.G, a.RT, reinterpret_cast<uint16_t*>(out)};
     const dim3 grid((unsigned)(H / 16));
     if (bf) hipLaunchKernelGGL((moe_owned_down_kernel<true, 3>), grid, dim3(64 * kOwnedWaves), 0, s, o);
     else hipLaunchKernelGGL((moe_owned_down_kernel<false, 3>), grid, dim3(64 * kOwnedWaves), 0, s, o);

@@ -27,20 +27,16 @@ struct Router {
   static constexpr int kWords = 2 * NSEG * kExperts + kExperts + 4;  // of scratch
   static constexpr int kIds = (64 * NSEG + 255) / 256;
 
-  // rows, groups of 16 and groups of 64 rows, counted in one word
+  // rows and groups of 64 rows, counted in one word
   __device__ __forceinline__ static uint32_t counts(int rows) {
-    return (uint32_t)rows | (uint32_t)((rows + 15) >> 4) << 11 | (uint32_t)((rows + 63) >> 6) << 22;
+    return (uint32_t)rows | (uint32_t)((rows + 63) >> 6) << 16;
   }
-  __device__ __forceinline__ static int row_at(uint32_t c) { return c & 0x7ff; }
-  template <int R>
-  __device__ __forceinline__ static int group_at(uint32_t c) {
-    static_assert(R == 16 || R == 64, "groups");
-    return R == 16 ? c >> 11 & 0x7ff : c >> 22;
-  }
+  __device__ __forceinline__ static int row_at(uint32_t c) { return c & 0xffff; }
+  __device__ __forceinline__ static int group_at(uint32_t c) { return c >> 16; }
 
   // The work-group's own token group, pick(groups) of the groups of 64 rows (-1: none), with
-  // its tokens, and the plan in groups of R rows from the first work-group.
-  template <int R, typename Pick>
+  // its tokens, and the plan from the first work-group.
+  template <typename Pick>
   __device__ __forceinline__ static bool here(const RouteArgs& a, uint32_t* scratch, TgEntry* own,
                                               int* tokens, Pick pick) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -94,20 +90,20 @@ struct Router {
       if (w < wave) at += total[w];
       all += total[w];
     }
-    const int g0 = pick(group_at<64>(all));
+    const int g0 = pick(group_at(all));
     const bool writer = blockIdx.x == 0;
-    if (writer && tid == 0) a.hdr[0] = group_at<R>(all);
+    if (writer && tid == 0) a.hdr[0] = group_at(all);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       if (k >= per || e0 + k >= a.E) break;
       first[e0 + k] = at;
-      const int g = g0 - group_at<64>(at);
+      const int g = g0 - group_at(at);
       if (g0 >= 0 && g >= 0 && g * 64 < cnt[k])
         *own = TgEntry{e0 + k, row_at(at) + g * 64, cnt[k] - g * 64 < 64 ? cnt[k] - g * 64 : 64, 2};
       if (writer)
-        for (int r = 0; r < cnt[k]; r += R)
-          a.tg[group_at<R>(at) + r / R] =
-              TgEntry{e0 + k, row_at(at) + r, cnt[k] - r < R ? cnt[k] - r : R, 2};
+        for (int r = 0; r < cnt[k]; r += 64)
+          a.tg[group_at(at) + r / 64] =
+              TgEntry{e0 + k, row_at(at) + r, cnt[k] - r < 64 ? cnt[k] - r : 64, 2};
       at += counts(cnt[k]);
     }
     __syncthreads();
@@ -121,7 +117,7 @@ struct Router {
       for (int w = 0; w < NSEG - 1; ++w)
         if (w < (i >> 6)) rank += __popcll(m[w]);
       if (writer) a.sorted[row_at(first[e]) + rank] = i;
-      if (group_at<64>(first[e]) + (rank >> 6) == g0) tokens[rank & 63] = i / a.top_k;
+      if (group_at(first[e]) + (rank >> 6) == g0) tokens[rank & 63] = i / a.top_k;
     }
     __syncthreads();
     return g0 >= 0;

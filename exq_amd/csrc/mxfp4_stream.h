@@ -12,10 +12,27 @@ namespace mx {
 // tile and the up tile of the same columns; the four waves of a work-group share its
 // contraction and add their sums through LDS in wave order.  A dropped slot reads the first
 // expert's weights and is not stored.  Bound: latency, the ids' and then the weights'.
-// Against the tiles that route first, 8 slots of 2048 x 768: 15.7 and 14.6 us a layer, 16 of
-// them 19.7 and 16.2, 32 22.7 and 23.7.
 constexpr int kSlotWaves = 4;
-constexpr int kSlotSlots = 16;       // up to which
+
+// Whether a layer of n slots runs by slots, with the down projection below, or routes and runs
+// on tiles.  Slots save the routing and a launch, tiles keep more of the weights on their way.
+// us a layer by slots and on tiles, weights not in the caches:
+//   1024 x 512   8 slots 11.2 and 16.7, 16 14.4 and 17.6, 24 18.3 and 19.3, 32 21.9 and 20.5
+//   2048 x 768   8 15.3 and 21.2, 16 20.5 and 23.9, 24 26.7 and 28.8, 32 31.4 and 30.8
+//   2048 x 2048  4 17.6 and 23.5, 8 25.3 and 26.0, 12 32.7 and 31.3, 16 40.4 and 33.9
+//   4096 x 1024  4 17.2 and 27.1, 8 21.5 and 28.6, 12 26.1 and 31.1, 16 33.2 and 33.3
+//   8192 x 1024  4 27.2 and 37.7, 8 36.0 and 41.2, 16 58.7 and 50.7
+//   4096 x 4096  2 25.0 and 37.6, 4 33.5 and 40.1, 8 54.5 and 52.6, 16 94.8 and 85.0
+//   6144 x 2048  2 28.1 and 35.0, 4 32.5 and 36.3, 8 52.4 and 43.7, 16 88.1 and 64.2
+//   4096 x 14336 2 67 and 83, 4 91 and 96, 8 162 and 143, 16 301 and 190
+//   8192 x 8192  1 59 and 84, 2 76 and 81, 3 90 and 84, 4 105 and 92, 8 188 and 157
+// So up to four slots, and up to 16 where all their experts' values are few.
+constexpr int kSlotSlots = 16;
+constexpr int kSlotAlways = 4;
+constexpr int64_t kSlotValues = (int64_t)3 << 24;     // slots x hidden x intermediate size
+inline bool runs_by_slot(int64_t slots, int64_t H, int64_t I) {
+  return slots <= kSlotAlways || (slots <= kSlotSlots && slots * H * I <= kSlotValues);
+}
 
 struct SlotArgs {
   const void* ids;           // [n]
@@ -95,19 +112,14 @@ __global__ void __launch_bounds__(64 * kSlotWaves) moe_slot_gateup_kernel(SlotAr
             pack16(silu_f32(v[0].z) * v[1].z, silu_f32(v[0].w) * v[1].w, BF)};
 }
 
-// ---- few slots: the down projection by output columns --------------------------------------
-// A work-group owns 16 output columns and takes every token group: wave w the groups w, w +
-// 8, ..., whose results it weighs into LDS, a row a slot; then a token's k rows are added in
-// the order of its slots.  No partial rows in memory and no launch to add them.  The rows
-// of mid are few and come straight from memory.  Against tiles and the combine launch, 16
-// slots of 768 x 2048: 19.5 and 21.1 us a layer, 32 22.7 and 23.4, 64 30.2 and 27.1.
+// ---- a few slots: the down projection by output columns ------------------------------------
+// A work-group owns 16 output columns and takes every slot: wave w the slots w, w + 8, ...,
+// whose results it weighs into LDS, a row a slot; then a token's k rows are added in the order
+// of its slots.  No partial rows in memory and no launch to add them.  The rows of mid are few
+// and come straight from memory.
 constexpr int kOwnedWaves = 8;
-constexpr int kOwnedSlots = 32;      // up to which
 
 struct OwnedArgs {
-  const int* hdr;            // null: every slot a group of its own
-  const TgEntry* tg;
-  const int* sorted;
   const uint16_t* mid;       // [n, I]
   const uint4* tiles;
   const uint8_t* wscales;
@@ -120,13 +132,12 @@ struct OwnedArgs {
 template <bool BF, int C>
 __global__ void __launch_bounds__(64 * kOwnedWaves) moe_owned_down_kernel(OwnedArgs a) {
   constexpr int W = kOwnedWaves;
-  __shared__ __align__(16) float rows[kOwnedSlots * 16];
-  __shared__ float wts[kOwnedSlots];
-  __shared__ int experts[kOwnedSlots];
+  __shared__ __align__(16) float rows[kSlotSlots * 16];
+  __shared__ float wts[kSlotSlots];
+  __shared__ int experts[kSlotSlots];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r16 = lane & 15, q = lane >> 4, n = a.T * a.k;
-  const int n_groups = a.hdr ? a.hdr[0] : n, blocks = a.I / kBlock;
+  const int r16 = lane & 15, q = lane >> 4, n = a.T * a.k, blocks = a.I / kBlock;
   if (tid < n) {   // (a dropped slot's weight is not looked at)
     const int64_t e = load_index(a.ids, a.ids_dtype, tid);
     const bool there = e >= 0 && e < a.E;
@@ -136,25 +147,16 @@ __global__ void __launch_bounds__(64 * kOwnedWaves) moe_owned_down_kernel(OwnedA
   for (int i = tid; i < n * 16; i += 64 * W) rows[i] = 0.f;
   __syncthreads();
   const int chunks = (a.KB + C - 1) / C;
-  const int items = n_groups > wave ? ((n_groups - wave + W - 1) / W) * chunks : 0;
+  const int items = n > wave ? ((n - wave + W - 1) / W) * chunks : 0;
   uint4 w[2][C], x[2][C][4];
   uint32_t s[2][C];
   int slot[2], li = 0;       // slot: the lane's row of the result, -1: none
   auto load = [&](int p) {
     const int i = li < items ? li : items - 1, gi = i / chunks, ch = i - gi * chunks;
-    TgEntry t;
-    if (a.hdr) {
-      t = a.tg[wave + gi * W];
-      slot[p] = r16 < t.cnt ? a.sorted[t.pos0 + r16] : -1;
-    } else {
-      t.pos0 = wave + gi * W;
-      t.e = experts[t.pos0];
-      t.cnt = t.e < 0 ? 0 : 1;
-      t.e = t.e < 0 ? 0 : t.e;
-      slot[p] = r16 < t.cnt ? t.pos0 : -1;
-    }
-    const int er = __builtin_amdgcn_readfirstlane(t.e);
-    const uint16_t* xr = a.mid + (int64_t)(t.pos0 + (r16 < t.cnt ? r16 : 0)) * a.I;
+    const int at = wave + gi * W, e = experts[at];
+    slot[p] = r16 == 0 && e >= 0 ? at : -1;
+    const int er = __builtin_amdgcn_readfirstlane(e < 0 ? 0 : e);
+    const uint16_t* xr = a.mid + (int64_t)at * a.I;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int kb = ch * C + c < a.KB ? ch * C + c : a.KB - 1;

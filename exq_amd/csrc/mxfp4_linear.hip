@@ -232,8 +232,13 @@ constexpr const char* kKernels[] = {"stream 16x16", "stream 32x16", "tile 32x128
 
 // `vec`: runs of the result and the residual may be stored and loaded at once.  Where they may
 // not, a tile's columns go one by one at its end, which the streams spread over more
-// work-groups (187 tokens x 1440 x 2047 with a residual: 32 x 128 tiles 15.7 us, 32 x 16
-// streams 12.3; x 2048 10.9 and 11.8).
+// work-groups: counted as 5 us of any tile.  In us with a residual, streams and tiles: bf16 100
+// x 1440 x 2047 8.0 and 12.2, 187 10.6 and 12.3, 400 x 512 x 1001 8.2 and 9.4, but 400 x 512 x
+// 2047 13.2 and 9.8, 187 x 4096 x 2047 26.8 and 19.3; MXFP4 187 x 1440 x 2047 7.2 and 10.2, 800
+// x 4096 x 14335 6 times the tiles' time.  Over 24 - 1600 tokens, K 512 - 4096 and 1001 - 14335
+// columns (168 calls) the choice is 0.5 % from the faster one in the mean, 22 % at most (187 x
+// 4096 x 2047 of MXFP4: 16.6 and 13.6); without the 5 us 4.4 and 76 %, by streams alone 56 % and
+// 7 times.
 constexpr int kUnalignedTileNs = 5000;
 
 int pick_kernel(int64_t tokens, int64_t rows, int64_t KB, bool x4, bool gated, bool vec) {

@@ -225,6 +225,7 @@ class _Workspaces(threading.local):
 
     def __init__(self):
         self.buffers = _Buffers()
+        self.by_key = self.buffers.by_key
         with _lock:
             _all_buffers.add(self.buffers)
 
@@ -234,9 +235,10 @@ _workspaces = _Workspaces()
 
 def _capturing(device: torch.device) -> bool:
     """Whether the device's current stream is being captured into a graph."""
-    if device.type != "cuda":
+    if not torch.cuda._initialized:   # (a third of what device.type takes)
         return False
-    if device.index is None or device.index == torch._C._cuda_getDevice():
+    index = device.index
+    if index is None or index == torch._C._cuda_getDevice():
         return torch._C._cuda_isCurrentStreamCapturing()
     with torch.cuda.device(device):
         return torch._C._cuda_isCurrentStreamCapturing()
@@ -250,9 +252,10 @@ def workspace(device: torch.device, nbytes: int, kind: str = "scratch",
     stream, and after a larger call has let go of a buffer that it holds the address of."""
     if _capturing(device):
         return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
-    key = (device.index if device.index is not None else torch.cuda.current_device(),
+    index = device.index
+    key = (torch.cuda.current_device() if index is None else index,
            stream_handle(device) if stream is None else stream, kind)
-    buffers = _workspaces.buffers.by_key
+    buffers = _workspaces.by_key
     buf = buffers.get(key)
     if buf is None or buf.numel() < nbytes:
         size = max(nbytes, 1 << 20)

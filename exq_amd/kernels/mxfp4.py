@@ -407,8 +407,7 @@ def fused_experts_mxfp4(hidden_states: torch.Tensor, w13: Mxfp4Weight, w2: Mxfp4
     if p.n_tokens == 0:
         return out
     if workspace is None:
-        workspace = _lib.workspace(out.device, need, "mxfp4",
-                                   torch._C._cuda_getCurrentRawStream(dev))
+        workspace = _scratch(out, dev, need)
     else:
         if (workspace.dtype != torch.uint8 or not workspace.is_contiguous()
                 or workspace.data_ptr() % 16):
@@ -421,6 +420,17 @@ def fused_experts_mxfp4(hidden_states: torch.Tensor, w13: Mxfp4Weight, w2: Mxfp4
                  a13, b13, a2, b2, out.data_ptr(), workspace.data_ptr(), workspace.numel()), dev,
                 "fused_experts_mxfp4")
     return out
+
+
+def _scratch(out: torch.Tensor, index: int, need: int) -> torch.Tensor:
+    """``_lib.workspace`` of out's device, which is the current one, with less Python where
+    the buffer is there (0.5 of a call's 13 us)."""
+    if not torch._C._cuda_isCurrentStreamCapturing():
+        stream = torch._C._cuda_getCurrentRawStream(index)
+        buf = _lib._workspaces.by_key.get((index, stream, "mxfp4"))
+        if buf is not None and buf.numel() >= need:
+            return buf
+    return _lib.workspace(out.device, need, "mxfp4")
 
 
 def moe_mxfp4_workspace_bytes(n_tokens: int, hidden: int, inter: int, n_experts: int,

@@ -8,10 +8,10 @@ namespace mx {
 
 // ---- a few slots: gate and up by slots -------------------------------------------------------
 // Every slot is a group of its own, so nothing has to be routed; experts that two tokens share
-// are read twice, from the caches.  A unit is a slot x a gate
-// tile and the up tile of the same columns; the four waves of a work-group share its
-// contraction and add their sums through LDS in wave order.  A dropped slot reads the first
-// expert's weights and is not stored.  Bound: latency, the ids' and then the weights'.
+// are read twice, from the caches.  A unit is a slot x a gate tile and the up tile of the same
+// columns; the four waves of a work-group share its contraction and add their sums through LDS
+// in wave order.  A dropped slot reads the first expert's weights and is not stored.  Bound:
+// latency, the ids' and then the weights' (1 x 8 of 2048 x 768 6.3 us, the down kernel 7.1).
 constexpr int kSlotWaves = 4;
 
 // Whether a layer of n slots runs by slots, with the down projection below, or routes and runs
